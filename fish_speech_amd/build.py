@@ -9,9 +9,9 @@ import time
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libfishmi.so")
-SOURCES = ["common.cpp", "dualar_kernels.hip", "dualar_gemm.hip", "dualar_attn.hip", "dualar_sample.hip", "dualar.hip",
+SOURCES = ["common.cpp", "dualar_kernels.hip", "dualar_gemm.hip", "dualar_attn.hip", "dualar_sample.hip", "kv4.hip", "dualar.hip",
            "dac_kernels.hip", "dac.hip"]
-HEADERS = ["common.h", "dualar_kernels.h", "dualar_dev.h", "dac_kernels.h", os.path.join("..", "..", "include", "fishmi.h")]
+HEADERS = ["common.h", "dualar_kernels.h", "dualar_dev.h", "kv4_kernels.h", "dac_kernels.h", os.path.join("..", "..", "include", "fishmi.h")]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Wno-unused-value", "-Wno-unused-result",
          # no packed fp32 arithmetic: the compiler forms v_pk_{add,mul,fma}_f32 from ordinary float code by itself, and some
          # of their forms have given wrong results on this part now and then (the host pass warns that it does not know

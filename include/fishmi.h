@@ -250,6 +250,80 @@ int fmi_op_sample(const void* logits_dev, int B, int n, int ld, const int32_t* i
                   const fmi_sampling* samp, int frame, int draw, const int32_t* prev_dev,
                   int sem_begin, int sem_end, int32_t* out_dev, void* stream);
 
+/* ---------------------------------------------------------------- 4-bit paged K/V cache -- */
+
+/* A K/V cache at 4.25 bits per value: a token of 8 kv heads x 128 dims takes 1 088 bytes for K and V instead of 4 096 in
+ * bf16.  The reference has only the cache in the model's own type (KVCache, llama.py:196-214); a model uses this one
+ * after fmi_dualar_set_kv_bits(h, 4), and these entry points offer it to other attention code.
+ *
+ * Values: 32 consecutive dims share a power of two 2^e, the smallest with max|x| <= 7 * 2^e (-100 <= e <= 125); a value is
+ * stored as the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times 2^e with its sign (ties to the even code, above 6 * 2^e reads
+ * as 6 * 2^e).  A block that holds an infinity or a NaN reads as 32 NaNs.
+ * Pool: uint8 [n_pages][n_kv_head][2 (K, V)][64 * (head_dim / 2 + head_dim / 32)]; a page holds 64 tokens: their code
+ * bytes (even dims in the low nibble), then their scale bytes (e + 127; 255 = NaN).  16-byte aligned.
+ * block_table_dev: int32 [n_seqs][max_pages], the page of tokens [64 i, 64 i + 64) of a sequence.  An id outside
+ * [0, n_pages) means "no page": appends to it are dropped, reads give 0 and attention does not see its keys.
+ * Sizes, strides and alignments are checked on the host, indices and lengths in device memory are checked by the
+ * kernels: no value in them makes a kernel leave the buffers. */
+typedef struct fmi_kv4_cache {
+  void* pool_dev;
+  const int32_t* block_table_dev;
+  int32_t n_pages, n_kv_head, head_dim /* 32, 64 or 128 */, n_seqs, max_pages;
+} fmi_kv4_cache;
+
+/* Bytes of one page of the pool; negative for an unsupported shape. */
+int64_t fmi_kv4_page_bytes(int n_kv_head, int head_dim);
+
+/* Rows of new tokens.  q / k / v: bf16, [heads][head_dim] contiguous within a row, rows `stride` elements apart (slices
+ * of a fused q|k|v projection do); 16-byte aligned.  In order, all optional: head RMSNorm of q and k (q_norm_dev /
+ * k_norm_dev, bf16 [head_dim], torch.nn.RMSNorm as llama.py:862-864), rotation of their first rope_dim dims (a multiple
+ * of 16; rope_dev = bf16 [rope_len][rope_dim / 2][2] cos, sin by position; pairs (2 i, 2 i + 1) as llama.py:1026-1038,
+ * or (i, i + rope_dim / 2) when rope_half); then k and v are stored and q goes to q_out_dev.
+ * Row r belongs to position row_pos_dev[r] of sequence row_seq_dev[r]; a row whose sequence is outside [0, n_seqs), or
+ * whose position is outside the block table or the rotation table, is padding: nothing of it is written.  A (sequence,
+ * position) pair may appear once per call. */
+typedef struct fmi_kv4_rows {
+  const void *q_dev, *k_dev, *v_dev;   /* q_dev NULL: keys and values only */
+  int64_t q_stride, k_stride, v_stride;
+  void* q_out_dev;                     /* bf16, may be q_dev itself only if no half-split rotation is asked for */
+  int64_t q_out_stride;
+  int32_t n_head;
+  const void *q_norm_dev, *k_norm_dev;
+  double norm_eps;
+  const void* rope_dev;
+  int32_t rope_len, rope_dim, rope_half;
+  const int32_t *row_seq_dev, *row_pos_dev;
+  int32_t rows;
+} fmi_kv4_rows;
+int fmi_op_kv4_append(const fmi_kv4_cache* cache, const fmi_kv4_rows* rows, void* stream);
+
+/* The stored values of `rows` (sequence, position) pairs: k_out / v_out bf16 [rows][n_kv_head][head_dim], exact.  Pairs
+ * outside the sequences, the block table or the pool read as 0. */
+int fmi_op_kv4_read(const fmi_kv4_cache* cache, const int32_t* row_seq_dev, const int32_t* row_pos_dev, int rows,
+                    void* k_out_dev, void* v_out_dev, void* stream);
+
+/* Causal attention over the cache (F.scaled_dot_product_attention, llama.py:928-934): sequence s has the query rows
+ * q_start_dev[s] .. q_start_dev[s + 1] - 1 (int32 [n_seqs + 1], ascending) at its last positions, row i of n at position
+ * kv_len_dev[s] - n + i, and sees the cached keys up to its own position; kv head = head / (n_head / n_kv_head).  fp32
+ * scores, softmax and sums, one rounding to bf16.  A row that sees no key gives 0; rows past the last sequence stay as
+ * they were.  max_q and max_kv bound the rows and keys of any sequence (they size the launch; rows beyond max_q of a
+ * sequence are not computed).  splits: key ranges a query tile is divided into, 1 .. 256, or 0 for a choice made from
+ * n_seqs, max_q and max_kv alone; with a fixed value a row's bits do not depend on the other sequences of the call. */
+typedef struct fmi_kv4_query {
+  const void* q_dev;
+  int64_t q_stride;
+  int32_t n_head;
+  const int32_t *q_start_dev, *kv_len_dev;
+  int32_t n_seqs, total_q, max_q, max_kv;
+  float scale;
+  int32_t splits;
+} fmi_kv4_query;
+/* Workspace fmi_op_kv4_attention needs for these sizes (0 for one key range); calls that may run at the same time need
+ * workspaces of their own.  Negative for bad sizes. */
+int64_t fmi_kv4_attention_ws_bytes(const fmi_kv4_cache* cache, const fmi_kv4_query* query);
+int fmi_op_kv4_attention(const fmi_kv4_cache* cache, const fmi_kv4_query* query, void* out_dev, int64_t out_stride,
+                         void* ws_dev, int64_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------------------------- codec (DAC) -- */
 
 typedef struct fmi_dac fmi_dac;

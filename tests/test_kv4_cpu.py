@@ -1,0 +1,199 @@
+"""The 4-bit K/V cache without a GPU: the number format's oracle, and every refusal of the C entry points and of the Python
+object (all of them are decided on the host before anything is launched)."""
+import ctypes as C
+import math
+
+import pytest
+import torch
+
+from fish_speech_amd import _lib, kv4
+from fish_speech_amd._lib import FishmiError, Kv4CacheC, Kv4QueryC, Kv4RowsC
+from oracle import kv4 as O
+
+A = 1 << 20   # an aligned address that is never dereferenced: every call below is refused first
+
+
+def test_representable_values_are_kept_and_ties_go_to_even_codes():
+    for e in (-100, -7, 0, 3, 100):
+        vals = torch.cat([O.GRID, -O.GRID, O.GRID, -O.GRID]) * 2.0 ** e
+        assert torch.equal(O.stored(vals), vals)
+    # borders between neighbours, next to a 6 that fixes the power
+    border = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0] + [6.0] * 25, dtype=torch.float64)
+    assert O.stored(border)[:7].tolist() == [0.0, 1.0, 1.0, 2.0, 2.0, 4.0, 4.0]
+
+
+def test_block_power_is_the_smallest_that_holds_the_largest_value():
+    for top, e in ((7.0, 0), (7.03125, 1), (3.5, -1), (3.515625, 0), (6.0, 0), (2.0 ** -90, -92), (2.0 ** -120, -100), (0.0, -100)):
+        y = torch.zeros(32, dtype=torch.float64)
+        y[5] = top
+        assert int(O.quantise(y)[1]) == e + 127, (top, e)
+
+
+def test_error_is_at_most_half_a_step():
+    g = torch.Generator().manual_seed(0)
+    y = torch.randn(400, 64, generator=g, dtype=torch.float64)
+    code, scale = O.quantise(y)
+    unit = torch.ldexp(torch.ones(400, 2, dtype=torch.float64), scale.long() - 127).repeat_interleave(32, 1)
+    a = y.abs() / unit
+    half = torch.where(a <= 2, 0.25, torch.where(a <= 4, 0.5, 1.0))
+    assert bool(((O.stored(y) - y).abs() <= half * unit).all())
+
+
+def test_nonfinite_blocks_read_as_nan_and_leave_their_neighbours():
+    y = torch.ones(1, 96)
+    y[0, 40] = math.inf
+    y[0, 70] = math.nan
+    s = O.stored(y)
+    assert s[0, :32].eq(1).all() and s[0, 32:].isnan().all()
+
+
+# ------------------------------------------------------------------------------------------------ refusals: C ABI
+
+
+def _cache(**kw):
+    d = dict(pool_dev=A, block_table_dev=A, n_pages=4, n_kv_head=2, head_dim=64, n_seqs=3, max_pages=5)
+    d.update(kw)
+    return Kv4CacheC(**d)
+
+
+def _rows(**kw):
+    d = dict(q_dev=A, k_dev=A, v_dev=A, q_stride=256, k_stride=128, v_stride=128, q_out_dev=A, q_out_stride=256, n_head=4,
+             norm_eps=1e-6, rope_dev=A, rope_len=10, rope_dim=64, row_seq_dev=A, row_pos_dev=A, rows=7)
+    d.update(kw)
+    return Kv4RowsC(**d)
+
+
+def _query(**kw):
+    d = dict(q_dev=A, q_stride=256, n_head=4, q_start_dev=A, kv_len_dev=A, n_seqs=3, total_q=5, max_q=2, max_kv=100,
+             scale=0.1, splits=1)
+    d.update(kw)
+    return Kv4QueryC(**d)
+
+
+BAD_CACHES = [dict(pool_dev=None), dict(pool_dev=A + 8), dict(block_table_dev=None), dict(block_table_dev=A + 2), dict(head_dim=48),
+              dict(head_dim=256), dict(n_pages=0), dict(n_kv_head=0), dict(n_kv_head=-1), dict(n_seqs=0), dict(max_pages=0),
+              dict(max_pages=(1 << 24) + 1)]
+
+
+@pytest.mark.parametrize("bad", BAD_CACHES, ids=str)
+def test_every_entry_point_refuses_a_bad_cache(bad):
+    lib = _lib.load()
+    c = C.byref(_cache(**bad))
+    assert lib.fmi_op_kv4_append(c, C.byref(_rows()), None) == -1
+    assert lib.fmi_op_kv4_read(c, A, A, 3, A, A, None) == -1
+    assert lib.fmi_op_kv4_attention(c, C.byref(_query()), A, 256, None, 0, None) == -1
+    assert b"kv4" in lib.fmi_last_error()
+
+
+@pytest.mark.parametrize("bad", [
+    dict(k_dev=None), dict(v_dev=None), dict(k_dev=A + 2), dict(v_stride=120), dict(v_stride=132), dict(k_stride=64),
+    dict(q_out_dev=None), dict(q_out_dev=A + 4), dict(q_stride=128), dict(q_out_stride=250), dict(n_head=0), dict(n_head=-4),
+    dict(row_seq_dev=None), dict(row_pos_dev=None), dict(rows=-1), dict(rope_dim=0), dict(rope_dim=8), dict(rope_dim=24),
+    dict(rope_dim=80), dict(rope_len=0), dict(rope_dev=A + 4), dict(q_norm_dev=A + 2), dict(k_norm_dev=A + 8),
+    dict(q_dev=None, q_norm_dev=A)], ids=str)
+def test_append_refusals(bad):
+    assert _lib.load().fmi_op_kv4_append(C.byref(_cache()), C.byref(_rows(**bad)), None) == -1
+
+
+@pytest.mark.parametrize("bad", [
+    dict(q_dev=None), dict(q_dev=A + 8), dict(q_stride=252), dict(q_stride=192), dict(n_head=0), dict(n_head=3), dict(q_start_dev=None),
+    dict(kv_len_dev=None), dict(n_seqs=-1), dict(n_seqs=4), dict(n_seqs=65536), dict(total_q=-1), dict(max_q=-1), dict(max_kv=-1),
+    dict(splits=-1), dict(splits=257)], ids=str)
+def test_attention_refusals(bad):
+    lib = _lib.load()
+    c, q = C.byref(_cache()), C.byref(_query(**bad))
+    assert lib.fmi_op_kv4_attention(c, q, A, 256, A, 1 << 30, None) == -1
+
+
+def test_attention_refuses_a_missing_or_small_workspace_and_bad_outputs():
+    lib = _lib.load()
+    c, q = C.byref(_cache()), C.byref(_query(splits=3))
+    need = lib.fmi_kv4_attention_ws_bytes(c, q)
+    assert need >= 3 * 5 * 4 * 64 * 4
+    assert lib.fmi_op_kv4_attention(c, q, A, 256, A, need - 1, None) == -1
+    assert lib.fmi_op_kv4_attention(c, q, A, 256, None, need, None) == -1
+    assert lib.fmi_op_kv4_attention(c, q, A, 256, A + 4, need, None) == -1
+    assert lib.fmi_op_kv4_attention(c, q, None, 256, A, need, None) == -1
+    assert lib.fmi_op_kv4_attention(c, q, A, 192, A, need, None) == -1
+    assert lib.fmi_kv4_attention_ws_bytes(c, C.byref(_query(splits=1))) == 0
+
+
+def test_null_arguments_and_empty_calls():
+    lib = _lib.load()
+    assert lib.fmi_op_kv4_append(None, C.byref(_rows()), None) == -1
+    assert lib.fmi_op_kv4_append(C.byref(_cache()), None, None) == -1
+    assert lib.fmi_op_kv4_read(None, A, A, 3, A, A, None) == -1
+    assert lib.fmi_op_kv4_read(C.byref(_cache()), None, A, 3, A, A, None) == -1
+    assert lib.fmi_op_kv4_read(C.byref(_cache()), A, A, -3, A, A, None) == -1
+    assert lib.fmi_op_kv4_read(C.byref(_cache()), A, A, 3, A + 2, A, None) == -1
+    assert lib.fmi_op_kv4_attention(None, C.byref(_query()), A, 256, None, 0, None) == -1
+    # nothing to do: fine, and nothing is launched
+    assert lib.fmi_op_kv4_append(C.byref(_cache()), C.byref(_rows(rows=0)), None) == 0
+    assert lib.fmi_op_kv4_read(C.byref(_cache()), None, None, 0, None, None, None) == 0
+    assert lib.fmi_op_kv4_attention(C.byref(_cache()), C.byref(_query(total_q=0)), A, 256, None, 0, None) == 0
+    assert lib.fmi_op_kv4_attention(C.byref(_cache()), C.byref(_query(n_seqs=0, q_start_dev=None, kv_len_dev=None)), A, 256,
+                                    None, 0, None) == 0
+
+
+def test_page_bytes():
+    assert kv4.page_bytes(8, 128) == 8 * 2 * 64 * (64 + 4)
+    assert kv4.page_bytes(2, 32) == 2 * 2 * 64 * (16 + 1)
+    for heads, dim in ((0, 128), (8, 96), (-1, 64)):
+        with pytest.raises(FishmiError):
+            kv4.page_bytes(heads, dim)
+
+
+# ------------------------------------------------------------------------------------------------ refusals: Python
+
+
+def test_cache_needs_a_gpu():
+    with pytest.raises(FishmiError, match="GPU"):
+        kv4.KV4Cache(4, 2, 64, device="cpu")
+
+
+@pytest.fixture
+def cache():
+    """A cache object whose tensors live on the CPU: good enough for checks that end before any launch."""
+    c = kv4.KV4Cache.__new__(kv4.KV4Cache)
+    c.lib, c.device = _lib.load(), torch.device("cpu")
+    c.n_pages, c.n_kv_head, c.head_dim = 4, 2, 64
+    c.pool = torch.zeros(4, 2, 2, 64 * 34, dtype=torch.uint8)
+    return c
+
+
+def _call(cache, what, **kw):
+    i32, bf = torch.int32, torch.bfloat16
+    a = dict(k=torch.zeros(3, 2, 64, dtype=bf), v=torch.zeros(3, 2, 64, dtype=bf), row_seq=torch.zeros(3, dtype=i32),
+             row_pos=torch.zeros(3, dtype=i32), block_table=torch.zeros(2, 3, dtype=i32))
+    if what == "attend":
+        a = dict(q=torch.zeros(3, 4, 64, dtype=bf), q_start=torch.zeros(3, dtype=i32), kv_len=torch.zeros(2, dtype=i32),
+                 block_table=torch.zeros(2, 3, dtype=i32), max_q=3, max_kv=10)
+    if what == "read":
+        a = {k: a[k] for k in ("row_seq", "row_pos", "block_table")}
+    a.update(kw)
+    return getattr(cache, what)(**a)
+
+
+BF = torch.bfloat16
+
+
+@pytest.mark.parametrize("what, kw", [
+    ("append", dict(k=torch.zeros(3, 2, 64))), ("append", dict(k=torch.zeros(3, 3, 64, dtype=BF))),
+    ("append", dict(v=torch.zeros(2, 2, 64, dtype=BF))), ("append", dict(v=torch.zeros(3, 2, 32, dtype=BF))),
+    ("append", dict(k=torch.zeros(3, 64, 2, dtype=BF).transpose(1, 2))), ("append", dict(row_seq=torch.zeros(3))),
+    ("append", dict(row_pos=torch.zeros(4, dtype=torch.int32))), ("append", dict(row_pos=torch.zeros(6, dtype=torch.int32)[::2])),
+    ("append", dict(block_table=torch.zeros(3, dtype=torch.int32))),
+    ("append", dict(block_table=torch.zeros(3, 2, dtype=torch.int32).t())),
+    ("append", dict(rope=torch.zeros(9, 32, 2))), ("append", dict(rope=torch.zeros(9, 64, dtype=BF))),
+    ("append", dict(rope=torch.zeros(9, 32, 2, dtype=BF), rope_layout="other")),
+    ("append", dict(k_norm=torch.zeros(32, dtype=BF))), ("append", dict(q_norm=torch.zeros(64, dtype=BF))),
+    ("append", dict(q_out=torch.zeros(3, 4, 64, dtype=BF))),
+    ("append", dict(q=torch.zeros(3, 4, 64, dtype=BF), q_out=torch.zeros(3, 5, 64, dtype=BF))),
+    ("attend", dict(q=torch.zeros(3, 4, 64))), ("attend", dict(q_start=torch.zeros(2, dtype=torch.int32))),
+    ("attend", dict(kv_len=torch.zeros(3, dtype=torch.int32))), ("attend", dict(kv_len=torch.zeros(2, dtype=torch.int64))),
+    ("attend", dict(out=torch.zeros(2, 4, 64, dtype=BF))),
+    ("read", dict(row_seq=torch.zeros(2, dtype=torch.int32))), ("read", dict(row_pos=torch.zeros(3, 1, dtype=torch.int32))),
+])
+def test_python_argument_errors(cache, what, kw):
+    with pytest.raises(ValueError):
+        _call(cache, what, **kw)
