@@ -75,6 +75,8 @@ _SIGS = {
     "fmi_dualar_finalize_weights": (C.c_int, [_P, _P]),
     "fmi_dualar_weights_ready": (C.c_int, [_P, _P]),
     "fmi_dualar_setup_caches": (C.c_int, [_P, _I, _I]),
+    "fmi_dualar_set_kv_bits": (C.c_int, [_P, _I]),
+    "fmi_dualar_read_kv4": (C.c_int, [_P, _I, _I, _I, _P, _P, _P]),
     "fmi_dualar_prefill": (C.c_int, [_P, _I, C.POINTER(C.c_int32), _P, C.POINTER(C.c_int32),
                                      C.POINTER(C.c_int32), C.POINTER(SamplingC), _P]),
     "fmi_dualar_prefill_resume": (C.c_int, [_P, _I, C.POINTER(C.c_int32), _P, C.POINTER(C.c_int32), C.POINTER(C.c_int32),

@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "dualar_kernels.h"
+#include "kv4_kernels.h"
 
 using namespace fmi;
 
@@ -68,6 +69,13 @@ struct fmi_dualar {
   hipEvent_t ev_in = nullptr, ev_out = nullptr, ev_t0 = nullptr, ev_t1 = nullptr;
   int max_batch = 0, max_seq = 0, n_pages = 0, max_pages = 0, max_frames = 0;
   std::vector<bf16_t*> kpool, vpool, fkc, fvc;
+  // kv_bits == 4 (fmi_dualar_set_kv_bits): the slow layers keep K and V in the 4-bit cache of kv4_kernels.h, one pool per
+  // layer in kv4_pool (kpool / vpool stay empty); the fast layers' ten keys stay bf16
+  int kv_bits = 16;
+  std::vector<uint8_t*> kv4_pool;
+  int32_t* kv4_seq = nullptr;   // prefill: [max_batch + 1] first rows, [max_batch] key counts, [max_batch] slots
+  int kv4_n = 0, kv4_max_q = 0; // its sequences and longest row range
+  float* kv4_part = nullptr;    // decode: partial states of the key ranges
   SlotState st{};
   std::vector<int> free_pages;
   std::vector<std::vector<int>> slot_pages;
@@ -347,12 +355,56 @@ int linear(fmi_dualar* h, const bf16_t* x, int ldx, const bf16_t* wp, const bf16
   return launch_linear_tiled(a, s);
 }
 
+// attention output projection and FFN of a slow block, after ws.ao holds the attention's output
+int block_slow_rest(fmi_dualar* h, const LayerW& w, bf16_t* x, int rows, hipStream_t s) {
+  const Dims& d = h->slow;
+  Workspace& ws = h->ws;
+  FMI_CHECK(linear(h, ws.ao, d.H * d.D, w.wo, nullptr, x, d.dim, x, d.dim, rows, d.dim, d.H * d.D, EPI_RESIDUAL, s, w.q_wo, w.s_wo, w.r_wo));
+  FMI_CHECK(linear(h, x, d.dim, w.w13, w.ffn_norm, nullptr, 0, ws.act, d.ffn, rows, 2 * d.ffn, d.dim, EPI_SILU, s, w.q_w13, w.s_w13));
+  FMI_CHECK(linear(h, ws.act, d.ffn, w.w2, nullptr, x, d.dim, x, d.dim, rows, d.dim, d.ffn, EPI_RESIDUAL, s, w.q_w2, w.s_w2, w.r_w2));
+  return FMI_OK;
+}
+
+// K/V append and attention over the 4-bit cache: ws.qkv -> ws.ao.  The key ranges of a decode step are a function of the
+// row's own position (kv4_attn_ranges under a fixed KV4_SPLITS) and prompts run in one range, so an utterance's numbers
+// do not depend on its batch-mates or on how its prompt was cut.
+constexpr int KV4_SPLITS = 16;
+int attn_kv4(fmi_dualar* h, const LayerW& w, int layer, int rows, const int32_t* row_slot, const int32_t* row_pos, hipStream_t s) {
+  const Dims& d = h->slow;
+  Workspace& ws = h->ws;
+  const Kv4Cache c{h->kv4_pool[layer], h->st.block_table, h->n_pages, d.KVH, d.D, h->max_batch, h->max_pages};
+  Kv4AppendArgs p{};
+  p.c = c; p.q = ws.qkv; p.k = ws.qkv + d.H * d.D; p.v = ws.qkv + (d.H + d.KVH) * d.D;
+  p.q_stride = p.k_stride = p.v_stride = d.qkv; p.q_out = ws.q; p.q_out_stride = d.H * d.D; p.H = d.H;
+  p.q_norm = h->cfg.attention_qk_norm ? w.q_norm : nullptr;
+  p.k_norm = h->cfg.attention_qk_norm ? w.k_norm : nullptr;
+  p.eps = h->cfg.norm_eps; p.rope = h->rope; p.rope_len = h->cfg.max_seq_len; p.rot = d.D;
+  p.row_seq = row_slot; p.row_pos = row_pos; p.slot_pos = h->st.pos; p.slot_done = row_pos ? nullptr : h->st.done; p.rows = rows;
+  FMI_CHECK(launch_kv4_append(p, s));
+  Kv4AttnArgs a{};
+  a.c = c; a.q = ws.q; a.out = ws.ao; a.q_stride = a.out_stride = d.H * d.D; a.slot_pos = h->st.pos; a.total_q = rows;
+  a.max_kv = h->max_seq; a.H = d.H; a.scale = 1.0f / sqrtf((float)d.D);
+  if (row_pos) {
+    a.q_start = h->kv4_seq; a.kv_len = h->kv4_seq + h->max_batch + 1; a.seq_slot = h->kv4_seq + 2 * h->max_batch + 1;
+    a.n_seqs = h->kv4_n; a.max_q = h->kv4_max_q; a.splits = 1;
+  } else {
+    a.seq_slot = row_slot; a.n_seqs = rows; a.max_q = 1; a.splits = KV4_SPLITS; a.part = h->kv4_part;
+  }
+  FMI_CHECK(launch_kv4_attn(a, s));
+  h->launches += a.splits > 1 ? 3 : 2;
+  return FMI_OK;
+}
+
 // one transformer block (llama.py:839-844) over `rows` rows of the residual stream x (in place)
 int block_slow(fmi_dualar* h, const LayerW& w, int layer, bf16_t* x, int rows, const int32_t* row_slot,
                const int32_t* row_pos, hipStream_t s) {
   const Dims& d = h->slow;
   Workspace& ws = h->ws;
   FMI_CHECK(linear(h, x, d.dim, w.wqkv, w.attn_norm, nullptr, 0, ws.qkv, d.qkv, rows, d.qkv, d.dim, EPI_STORE, s, w.q_wqkv, w.s_wqkv, w.r_wqkv));
+  if (h->kv_bits == 4) {
+    FMI_CHECK(attn_kv4(h, w, layer, rows, row_slot, row_pos, s));
+    return block_slow_rest(h, w, x, rows, s);
+  }
   AttnArgs a{};
   a.qkv = ws.qkv; a.q = ws.q; a.out = ws.ao; a.kpool = h->kpool[layer]; a.vpool = h->vpool[layer];
   a.qnw = h->cfg.attention_qk_norm ? w.q_norm : nullptr;
@@ -378,10 +430,7 @@ int block_slow(fmi_dualar* h, const LayerW& w, int layer, bf16_t* x, int rows, c
     else FMI_CHECK(launch_attn(a, s));
     h->launches += 2;
   }
-  FMI_CHECK(linear(h, ws.ao, d.H * d.D, w.wo, nullptr, x, d.dim, x, d.dim, rows, d.dim, d.H * d.D, EPI_RESIDUAL, s, w.q_wo, w.s_wo, w.r_wo));
-  FMI_CHECK(linear(h, x, d.dim, w.w13, w.ffn_norm, nullptr, 0, ws.act, d.ffn, rows, 2 * d.ffn, d.dim, EPI_SILU, s, w.q_w13, w.s_w13));
-  FMI_CHECK(linear(h, ws.act, d.ffn, w.w2, nullptr, x, d.dim, x, d.dim, rows, d.dim, d.ffn, EPI_RESIDUAL, s, w.q_w2, w.s_w2, w.r_w2));
-  return FMI_OK;
+  return block_slow_rest(h, w, x, rows, s);
 }
 
 // merge01 (tail): x holds 2 B rows -- rows [0, B) the B utterances at fast position 0, rows [B, 2B) the same utterances
@@ -696,12 +745,13 @@ void fmi_dualar_destroy(fmi_dualar* h) {
   free_ws(h->ws);
   for (auto p : h->kpool) hipFree(p);
   for (auto p : h->vpool) hipFree(p);
+  for (auto p : h->kv4_pool) hipFree(p);
   for (auto p : h->fkc) hipFree(p);
   for (auto p : h->fvc) hipFree(p);
   void* ptrs[] = {h->st.pos, h->st.frame, h->st.done, h->st.limit, h->st.cur, h->st.window, h->st.out,
                   h->st.temperature, h->st.top_p, h->st.top_k, h->st.seed, h->st.use_ras, h->st.block_table,
                   h->hn, h->hf, h->xl, h->xf, h->logits, h->flogits, h->ftrace, h->staging, h->staging2,
-                  h->qkv0_tab, h->qkv0_pre, h->attn_part, h->hfp, h->x01, h->gemm_part};
+                  h->qkv0_tab, h->qkv0_pre, h->attn_part, h->hfp, h->x01, h->gemm_part, h->kv4_seq, h->kv4_part};
   for (void* p : ptrs)
     if (p) hipFree(p);
   for (void* p : h->row_copies) hipFree(p);
@@ -930,7 +980,16 @@ int fmi_dualar_setup_caches(fmi_dualar* h, int max_batch, int max_seq_len) {
   h->n_pages = h->max_pages * max_batch;
   h->max_frames = max_seq_len;
   const int ncb1 = c.num_codebooks + 1;
-  for (int i = 0; i < c.n_layer; ++i) {
+  if (h->kv_bits == 4) {
+    for (int i = 0; i < c.n_layer; ++i) {
+      uint8_t* p;
+      FMI_CHECK(dev_alloc(&p, (int64_t)h->n_pages * s.KVH * 2 * kv4_block_bytes(s.D)));
+      h->kv4_pool.push_back(p);
+    }
+    FMI_CHECK(dev_alloc(&h->kv4_seq, (int64_t)3 * max_batch + 1));
+    FMI_CHECK(dev_alloc(&h->kv4_part, kv4_attn_part_floats(max_batch, s.H, s.D, KV4_SPLITS)));
+  }
+  for (int i = 0; i < c.n_layer && h->kv_bits == 16; ++i) {
     bf16_t *k, *v;
     FMI_CHECK(dev_alloc(&k, (int64_t)h->n_pages * s.KVH * KV_PAGE * s.D));
     FMI_CHECK(dev_alloc(&v, (int64_t)h->n_pages * s.KVH * KV_PAGE * s.D));
@@ -983,10 +1042,36 @@ int fmi_dualar_setup_caches(fmi_dualar* h, int max_batch, int max_seq_len) {
   {
     static const int env_thr = []() { const char* e = getenv("FMI_ATTN_THR"); return e ? atoi(e) : -1; }();
     if (env_thr >= 0) h->attn_long_thr = env_thr;
-    if (!attn_decode_long_supported(s.H, s.KVH, s.D)) h->attn_long_thr = 0;
+    if (!attn_decode_long_supported(s.H, s.KVH, s.D) || h->kv_bits == 4) h->attn_long_thr = 0;
     if (h->attn_long_thr > 0) FMI_CHECK(dev_alloc(&h->attn_part, attn_decode_long_part_floats(max_batch, s.H, s.D)));
   }
   return ensure_rows(h, std::max(max_batch, std::min(32, 2 * max_batch)));   // the merged fast pass runs 2 B <= 32 rows
+}
+
+int fmi_dualar_set_kv_bits(fmi_dualar* h, int bits) {
+  FMI_REQUIRE(h, "null handle");
+  FMI_REQUIRE(bits == 16 || bits == 4, "K/V cache of %d bits (16 or 4)", bits);
+  if (h->max_batch > 0 && bits != h->kv_bits)
+    return set_error(FMI_ESTATE, "the K/V cache's type is fixed once setup_caches has run");
+  h->kv_bits = bits;
+  return FMI_OK;
+}
+
+int fmi_dualar_read_kv4(fmi_dualar* h, int layer, int slot, int n, void* k_out_dev, void* v_out_dev, void* stream) {
+  FMI_REQUIRE(h, "null handle");
+  FMI_CHECK(check_slot(h, slot));
+  FMI_REQUIRE(h->kv_bits == 4, "the cache is not held in 4 bits");
+  FMI_REQUIRE(layer >= 0 && layer < h->cfg.n_layer, "layer %d out of range [0,%d)", layer, h->cfg.n_layer);
+  FMI_REQUIRE(n >= 0 && n <= (int)h->slot_pages[slot].size() * KV_PAGE, "slot %d holds pages for %d tokens, %d asked for", slot,
+              (int)h->slot_pages[slot].size() * KV_PAGE, n);
+  if (n == 0) return FMI_OK;
+  FMI_REQUIRE(k_out_dev && v_out_dev, "null argument");
+  FMI_CHECK(sync_in(h, stream));
+  Kv4ReadArgs a{};
+  a.c = Kv4Cache{h->kv4_pool[layer], h->st.block_table, h->n_pages, h->slow.KVH, h->slow.D, h->max_batch, h->max_pages};
+  a.seq0 = slot; a.rows = n; a.k = (bf16_t*)k_out_dev; a.v = (bf16_t*)v_out_dev;
+  FMI_CHECK(launch_kv4_read(a, h->stream));
+  return sync_out(h, stream);
 }
 
 int fmi_dualar_release(fmi_dualar* h, int slot) {
@@ -1060,6 +1145,17 @@ static int prefill_impl(fmi_dualar* h, int n, const int32_t* slot_ids, const int
   // causal work grows with the tile's position: heaviest query tiles first
   std::stable_sort(tiles.begin(), tiles.end(), [](const int4& x, const int4& y) { return x.w > y.w; });
   ws.n_qtiles = (int)tiles.size();
+  std::vector<int32_t> kv4_seq(3 * h->max_batch + 1, 0);
+  if (h->kv_bits == 4) {
+    h->kv4_n = n;
+    h->kv4_max_q = *std::max_element(lens, lens + n);
+    for (int i = 0; i < n; ++i) {
+      kv4_seq[i + 1] = kv4_seq[i] + lens[i];
+      kv4_seq[h->max_batch + 1 + i] = (pos0 ? pos0[i] : 0) + lens[i];
+      kv4_seq[2 * h->max_batch + 1 + i] = slot_ids[i];
+    }
+    FMI_CHECK_HIP(hipMemcpyAsync(h->kv4_seq, kv4_seq.data(), kv4_seq.size() * 4, hipMemcpyHostToDevice, s));
+  }
   FMI_CHECK_HIP(hipMemcpyAsync(ws.qtiles, tiles.data(), tiles.size() * sizeof(int4), hipMemcpyHostToDevice, s));
   FMI_CHECK_HIP(hipStreamSynchronize(s));  // host vectors go out of scope
   h->launches = 0;

@@ -240,7 +240,7 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadArgs a) {
   const int head = (int)(w % heads), isv = head & 1, kh = head >> 1;
   const int64_t row = (w / heads) * RPW + lane / LPH;
   if (row >= a.rows) return;
-  const int seq = a.row_seq[row], pos = a.row_pos[row];
+  const int seq = a.row_seq ? a.row_seq[row] : a.seq0, pos = a.row_seq ? a.row_pos[row] : (int)row;
   u32x4 x = {0, 0, 0, 0};
   if (seq >= 0 && seq < a.c.n_slots && pos >= 0 && pos < (int64_t)a.c.max_pages * KV_PAGE) {
     const int page = a.c.block_table[(int64_t)seq * a.c.max_pages + pos / KV_PAGE];
@@ -259,7 +259,7 @@ int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s) {
   FMI_REQUIRE(a.rows >= 0, "kv4 read: negative row count");
   if (a.rows == 0) return FMI_OK;
   const int D = a.c.D;
-  FMI_REQUIRE(a.row_seq && a.row_pos, "kv4 read: null row indices");
+  FMI_REQUIRE(!a.row_seq == !a.row_pos, "kv4 read: null row indices");
   FMI_CHECK(kv4_check_rows("k", a.k, (int64_t)a.c.KVH * D, a.c.KVH, D));
   FMI_CHECK(kv4_check_rows("v", a.v, (int64_t)a.c.KVH * D, a.c.KVH, D));
   const int rpw = 64 / (D / 8);
@@ -278,8 +278,8 @@ int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s) {
 //
 // out[row][head] = sum_key softmax_key(scale * q . k) v over the keys [0, pos(row)] of the row's sequence; a row
 // without keys gives 0.  A work-group of 4 waves owns a tile of 16 query columns of one sequence and kv head -- column =
-// (query row, head of the kv head's group), so K and V are read once for all of them -- and one of `splits` ranges of
-// 32-key blocks; wave w takes blocks w, w + 4, ... of the range.  Per block:
+// (query row, head of the kv head's group), so K and V are read once for all of them -- and one of up to `splits` ranges
+// of 32-key blocks; wave w takes blocks w, w + 4, ... of the range.  Per block:
 //   scores   S^T = K Q^T, v_mfma_f32_16x16x32_bf16: lane (c, g) holds the D / 4 dims from g D / 4 of key c, which is one
 //            consecutive piece of the page and one scale; Q is read in the same order, so no dim is moved;
 //   softmax  fp32, online, per column; the probabilities stay in registers as the B operand of the next product, split
@@ -302,6 +302,15 @@ __device__ inline Kv4Span kv4_span(const Kv4AttnArgs& a, int s) {
   r.kv = min(max(a.kv_len ? a.kv_len[s] : a.slot_pos[r.slot] + 1, 0), 1 << 30);
   r.cached = (int)min((int64_t)r.kv, (int64_t)a.c.max_pages * KV_PAGE);
   return r;
+}
+
+// the ranges a tile of nb key blocks really uses, at least 8 blocks (256 keys) each: a function of the tile alone.  One
+// range: its work-group writes the output itself and the merge passes the tile's rows by.
+__device__ inline int kv4_attn_ranges(int nb, int splits) { return max(1, min(splits, nb / 8)); }
+// key blocks of 32 that the tile of 16 columns from col0 sees
+__device__ inline int kv4_tile_blocks(const Kv4Span& sp, int G, int col0) {
+  const int nk = min(sp.kv - sp.nq + min(col0 + 15, sp.nq * G - 1) / G + 1, sp.cached);
+  return nk > 0 ? (nk + 31) / 32 : 0;
 }
 
 template <int D>
@@ -327,9 +336,9 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
   const int col = min(col0 + c, cols - 1);
   const int qrow = sp.row0 + col / G, head = kvh * G + col % G, qpos = pos0 + col / G;
   const int vis = min(qpos + 1, sp.cached);      // keys [0, vis) are this column's
-  const int nk = min(pos0 + min(col0 + 15, cols - 1) / G + 1, sp.cached);
-  const int nb = nk > 0 ? (nk + KB - 1) / KB : 0;
-  const int b_lo = (int)((int64_t)z * nb / a.splits), b_hi = (int)((int64_t)(z + 1) * nb / a.splits);
+  const int nb = kv4_tile_blocks(sp, G, col0), nz = kv4_attn_ranges(nb, a.splits);
+  if (z >= nz) return;
+  const int b_lo = (int)((int64_t)z * nb / nz), b_hi = (int)((int64_t)(z + 1) * nb / nz);
   const int32_t* bt = a.c.block_table + (int64_t)sp.slot * a.c.max_pages;
 
   bf16x8 qf[KS];                                 // B operand: column c, dims g D / 4 + 8 kk ..
@@ -480,7 +489,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
     const int v = min(pos0 + row + 1, sp.cached);
     if (bad < v) O = __uint_as_float(0x7fc00000u);
     const int64_t idx = (int64_t)(sp.row0 + row) * a.H + hd;
-    if (a.splits == 1) {
+    if (nz == 1) {
       a.out[(sp.row0 + row) * a.out_stride + (int64_t)hd * D + d] = L != 0.f ? f2bf(O / L) : (bf16_t)0;
     } else {
       float* part = a.part + ((int64_t)z * a.total_q * a.H + idx) * (D + 2);
@@ -501,12 +510,15 @@ __global__ __launch_bounds__(128) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
   const int i = blockIdx.x * 2 + (threadIdx.x >> 6);
   const int row = i / a.H, hd = i % a.H;
   if (row >= sp.nq) return;
+  const int G = a.H / a.c.KVH;
+  const int nz = kv4_attn_ranges(kv4_tile_blocks(sp, G, (row * G + hd % G) & ~15), a.splits);
+  if (nz == 1) return;
   const int64_t step = (int64_t)a.total_q * a.H * (D + 2);
   const float* part = a.part + ((int64_t)(sp.row0 + row) * a.H + hd) * (D + 2);
   float M = -FLT_MAX;
-  for (int z = 0; z < a.splits; ++z) M = fmaxf(M, part[z * step]);
+  for (int z = 0; z < nz; ++z) M = fmaxf(M, part[z * step]);
   float L = 0.f, O[D > 64 ? 2 : 1] = {};
-  for (int z = 0; z < a.splits; ++z) {
+  for (int z = 0; z < nz; ++z) {
     const float wgt = __builtin_amdgcn_exp2f(part[z * step] - M);
     L += part[z * step + 1] * wgt;
 #pragma unroll
@@ -591,6 +603,7 @@ int fmi_op_kv4_append(const fmi_kv4_cache* cache, const fmi_kv4_rows* r, void* s
 int fmi_op_kv4_read(const fmi_kv4_cache* cache, const int32_t* row_seq_dev, const int32_t* row_pos_dev, int rows,
                     void* k_out_dev, void* v_out_dev, void* stream) {
   FMI_REQUIRE(cache, "null argument");
+  FMI_REQUIRE(rows == 0 || (row_seq_dev && row_pos_dev), "kv4 read: null row indices");
   Kv4ReadArgs a{};
   a.c = kv4_cache_of(*cache);
   a.row_seq = row_seq_dev; a.row_pos = row_pos_dev; a.rows = rows; a.k = (bf16_t*)k_out_dev; a.v = (bf16_t*)v_out_dev;

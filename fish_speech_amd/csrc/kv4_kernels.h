@@ -36,7 +36,8 @@ int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s);
 
 struct Kv4ReadArgs {
   Kv4Cache c;
-  const int32_t *row_seq, *row_pos;
+  const int32_t *row_seq, *row_pos;         // row_seq == nullptr: row r = position r of sequence seq0
+  int seq0;
   int rows;
   bf16_t *k, *v;                            // [rows][KVH][D]
 };
@@ -53,10 +54,10 @@ struct Kv4AttnArgs {
   const int32_t* slot_pos;
   int n_seqs, total_q, max_q, max_kv, H;
   float scale;
-  int splits;                               // key ranges per query tile (kv4_attn_splits), >= 1
+  int splits;                               // most key ranges per query tile (kv4_attn_splits), >= 1
   float* part;                              // splits > 1: kv4_attn_part_floats
 };
-// key ranges a call of these sizes is split into: a function of the host's sizes only
+// most key ranges a call of these sizes is split into: a function of the host's sizes only
 int kv4_attn_splits(int n_seqs, int max_q, int max_kv, int H, int KVH);
 int64_t kv4_attn_part_floats(int total_q, int H, int D, int splits);
 int launch_kv4_attn(const Kv4AttnArgs& a, hipStream_t s);

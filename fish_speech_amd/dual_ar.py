@@ -222,6 +222,7 @@ class MiDualAR:
         self._cache_setup_done = False
         self.max_batch_size = -1
         self.max_seq_len = -1
+        self.kv_bits = 16
         self._frame_index = 0
         self._ignore_eos = False
         self._cached_prompt: Dict[int, torch.Tensor] = {}   # slot -> prompt columns whose prefill K/V it still holds
@@ -365,11 +366,23 @@ class MiDualAR:
         return model.load_state_dict(weights, strict=False)
 
     # ---- caches (llama.py:307-324,708-722)
-    def setup_caches(self, max_batch_size: int, max_seq_len: int, dtype: torch.dtype = torch.bfloat16):
+    def setup_caches(self, max_batch_size: int, max_seq_len: int, dtype: torch.dtype = torch.bfloat16,
+                     kv_bits: Optional[int] = None):
+        """``kv_bits=4``: the slow transformer's K/V cache in 4-bit floats (fishmi.h: fmi_dualar_set_kv_bits), 3.76 times
+        the slots or the context in the same memory; logits then carry that rounding.  16 = bf16; None keeps what an
+        earlier call chose (bf16 on the first)."""
         if dtype != torch.bfloat16:
-            raise _lib.FishmiError("only bfloat16 KV caches are implemented")
+            raise _lib.FishmiError("only bfloat16 KV caches are implemented (and the 4-bit form of kv_bits=4)")
+        if kv_bits is None:
+            kv_bits = self.kv_bits
+        if kv_bits not in (16, 4):
+            raise ValueError(f"kv_bits {kv_bits}: 16 or 4")
+        if self._cache_setup_done and kv_bits != self.kv_bits:
+            raise _lib.FishmiError(f"the K/V cache is already set up with {self.kv_bits} bits")
         if self.max_seq_len >= max_seq_len and self.max_batch_size >= max_batch_size:
             return
+        check(self.lib.fmi_dualar_set_kv_bits(self._h, int(kv_bits)))
+        self.kv_bits = kv_bits
         check(self.lib.fmi_dualar_setup_caches(self._h, int(max_batch_size), int(max_seq_len)))
         self.max_batch_size, self.max_seq_len = max_batch_size, max_seq_len
         self._cache_setup_done = True
@@ -568,6 +581,15 @@ class MiDualAR:
         """Keep generating past <|im_end|> (fixed-length synthetic benchmarks)."""
         check(self.lib.fmi_dualar_set_ignore_eos(self._h, int(enable)))
         self._ignore_eos = bool(enable)
+
+    def read_kv4(self, layer: int, slot: int, n: int):
+        """K and V of a slot's positions [0, n) in one slow layer as the 4-bit cache holds them (after head norm and
+        rotation): bf16 (n, n_local_heads, head_dim) each.  Needs ``setup_caches(..., kv_bits=4)``."""
+        cfg = self.config
+        k, v = (torch.empty(n, cfg.n_local_heads, cfg.head_dim, dtype=torch.bfloat16, device=self.device) for _ in range(2))
+        check(self.lib.fmi_dualar_read_kv4(self._h, int(layer), int(slot), int(n), C.c_void_p(k.data_ptr()),
+                                           C.c_void_p(v.data_ptr()), self._stream()))
+        return k, v
 
     # ---- parity taps
     def debug_taps(self, B: int = 1):

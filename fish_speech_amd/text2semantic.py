@@ -166,9 +166,9 @@ def init_model(checkpoint_path, device, precision=torch.bfloat16, compile: bool 
     return model.eval(), decode_one_token
 
 
-def launch_thread_safe_queue(checkpoint_path, device, precision=torch.bfloat16, compile: bool = False):
+def launch_thread_safe_queue(checkpoint_path, device, precision=torch.bfloat16, compile: bool = False, kv_bits: int = 16):
     """One worker thread owns the model and serves GenerateRequests from the returned queue; `None` stops it
-    (inference.py:748-799).  Errors travel back as WrappedGenerateResponse("error", exception)."""
+    (inference.py:748-799).  ``kv_bits=4`` keeps the K/V cache in 4-bit floats.  Errors travel back as WrappedGenerateResponse("error", exception)."""
     input_queue: queue.Queue = queue.Queue()
     ready = threading.Event()
     failure: List[BaseException] = []
@@ -177,7 +177,7 @@ def launch_thread_safe_queue(checkpoint_path, device, precision=torch.bfloat16, 
         try:
             model, decode_one_token = init_model(checkpoint_path, device, precision, compile=compile)
             model.setup_caches(max_batch_size=1, max_seq_len=model.config.max_seq_len,
-                               dtype=next(iter(model.parameters())).dtype)
+                               dtype=next(iter(model.parameters())).dtype, kv_bits=kv_bits)
         except BaseException as e:   # surface load failures to the caller instead of hanging it
             failure.append(e)
             ready.set()
@@ -223,8 +223,9 @@ def _cli():
     @click.option("--iterative-prompt/--no-iterative-prompt", default=True)
     @click.option("--chunk-length", type=int, default=300)
     @click.option("--output-dir", type=Path, default="output")
+    @click.option("--kv-bits", type=click.Choice(["16", "4"]), default="16", help="K/V cache in bf16 or in 4-bit floats")
     def main(text, prompt_text, prompt_tokens, prompt_audio, output, num_samples, max_new_tokens, top_p, top_k,
-             temperature, checkpoint_path, device, compile, seed, half, iterative_prompt, chunk_length, output_dir):
+             temperature, checkpoint_path, device, compile, seed, half, iterative_prompt, chunk_length, output_dir, kv_bits):
         """Text -> codes_N.npy (and a wav with --output); flags of fish_speech/models/text2semantic/inference.py:802-838."""
         os.makedirs(output_dir, exist_ok=True)
         if half:
@@ -237,7 +238,7 @@ def _cli():
             raise ValueError(f"Number of prompt text ({len(prompt_text)}) and prompt audio ({len(prompt_audio)}) should be the same")
         t0 = time.time()
         model, decode_one_token = init_model(checkpoint_path, device, torch.bfloat16, compile=compile)
-        model.setup_caches(max_batch_size=1, max_seq_len=model.config.max_seq_len)
+        model.setup_caches(max_batch_size=1, max_seq_len=model.config.max_seq_len, kv_bits=int(kv_bits))
         print(f"Time to load model: {time.time() - t0:.02f} seconds")
 
         codec = None

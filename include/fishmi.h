@@ -86,6 +86,15 @@ int fmi_dualar_weights_ready(fmi_dualar* h, void* stream);
 /* KV-cache page pool + per-slot state for up to max_batch concurrent utterances of up to
  * max_seq_len positions.  Replaces DualARTransformer.setup_caches (llama.py:307-324,708-722). */
 int fmi_dualar_setup_caches(fmi_dualar* h, int max_batch, int max_seq_len);
+/* Type of the slow transformer's K/V cache: 16 = bf16 as the reference (default), 4 = the 4-bit cache described at
+ * fmi_kv4_cache below: 39 168 bytes per token instead of 147 456 at 36 layers of 8 kv heads x 128 dims, for 3.76 times the
+ * slots or the context in the same memory.  Keys and values then carry the rounding of that format (every query attends
+ * to the stored values, also to its own token's), so logits and tokens differ from a bf16 cache's.  Call before
+ * fmi_dualar_setup_caches. */
+int fmi_dualar_set_kv_bits(fmi_dualar* h, int bits);
+/* The stored K and V of positions [0, n) of a slot in one slow layer (4-bit cache only): bf16 [n][n_local_heads][head_dim]
+ * each, after norm and rotation.  Pages of released slots may have been reused. */
+int fmi_dualar_read_kv4(fmi_dualar* h, int layer, int slot, int n, void* k_out_dev, void* v_out_dev, void* stream);
 
 typedef struct fmi_sampling {
   float temperature, top_p; /* rounded to bf16 inside, like inference.py:305-306 */
