@@ -41,26 +41,6 @@ class DacConfigC(C.Structure):
                 ("enc_tf_window", C.c_int32), ("sample_rate", C.c_int32)]
 
 
-class Kv4CacheC(C.Structure):
-    _fields_ = [("pool_dev", C.c_void_p), ("block_table_dev", C.c_void_p), ("n_pages", C.c_int32),
-                ("n_kv_head", C.c_int32), ("head_dim", C.c_int32), ("n_seqs", C.c_int32), ("max_pages", C.c_int32)]
-
-
-class Kv4RowsC(C.Structure):
-    _fields_ = [("q_dev", C.c_void_p), ("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("q_stride", C.c_int64),
-                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_dev", C.c_void_p),
-                ("q_out_stride", C.c_int64), ("n_head", C.c_int32), ("q_norm_dev", C.c_void_p),
-                ("k_norm_dev", C.c_void_p), ("norm_eps", C.c_double), ("rope_dev", C.c_void_p),
-                ("rope_len", C.c_int32), ("rope_dim", C.c_int32), ("rope_half", C.c_int32),
-                ("row_seq_dev", C.c_void_p), ("row_pos_dev", C.c_void_p), ("rows", C.c_int32)]
-
-
-class Kv4QueryC(C.Structure):
-    _fields_ = [("q_dev", C.c_void_p), ("q_stride", C.c_int64), ("n_head", C.c_int32), ("q_start_dev", C.c_void_p),
-                ("kv_len_dev", C.c_void_p), ("n_seqs", C.c_int32), ("total_q", C.c_int32), ("max_q", C.c_int32),
-                ("max_kv", C.c_int32), ("scale", C.c_float), ("splits", C.c_int32)]
-
-
 _P = C.c_void_p
 _I = C.c_int
 _SIGS = {
@@ -108,10 +88,11 @@ _SIGS = {
     "fmi_op_linear_bf16": (C.c_int, [_P, _P, _P, _P, _P, _I, _I, _I, C.c_float, _I, _I, _P]),
     "fmi_op_sample": (C.c_int, [_P, _I, _I, _I, _P, C.POINTER(SamplingC), _I, _I, _P, _I, _I, _P, _P]),
     "fmi_kv4_page_bytes": (C.c_int64, [_I, _I]),
-    "fmi_op_kv4_append": (C.c_int, [C.POINTER(Kv4CacheC), C.POINTER(Kv4RowsC), _P]),
-    "fmi_op_kv4_read": (C.c_int, [C.POINTER(Kv4CacheC), _P, _P, _I, _P, _P, _P]),
-    "fmi_kv4_attention_ws_bytes": (C.c_int64, [C.POINTER(Kv4CacheC), C.POINTER(Kv4QueryC)]),
-    "fmi_op_kv4_attention": (C.c_int, [C.POINTER(Kv4CacheC), C.POINTER(Kv4QueryC), _P, C.c_int64, _P, C.c_int64, _P]),
+    # (fmi_kv4_cache / fmi_kv4_rows / fmi_kv4_query are passed as packed bytes: kv4.py)
+    "fmi_op_kv4_append": (C.c_int, [_P, _P, _P]),
+    "fmi_op_kv4_read": (C.c_int, [_P, _P, _P, _I, _P, _P, _P]),
+    "fmi_kv4_attention_ws_bytes": (C.c_int64, [_P, _P]),
+    "fmi_op_kv4_attention": (C.c_int, [_P, _P, _P, C.c_int64, _P, C.c_int64, _P]),
     "fmi_dac_arena_bytes": (C.c_int64, [C.POINTER(DacConfigC)]),
     "fmi_dac_create": (C.c_int, [C.POINTER(DacConfigC), _P, C.c_int64, C.POINTER(_P)]),
     "fmi_dac_destroy": (None, [_P]),

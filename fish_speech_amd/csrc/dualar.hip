@@ -366,8 +366,8 @@ int block_slow_rest(fmi_dualar* h, const LayerW& w, bf16_t* x, int rows, hipStre
 }
 
 // K/V append and attention over the 4-bit cache: ws.qkv -> ws.ao.  The key ranges of a decode step are a function of the
-// row's own position (kv4_attn_ranges under a fixed KV4_SPLITS) and prompts run in one range, so an utterance's numbers
-// do not depend on its batch-mates or on how its prompt was cut.
+// row's own position (kv4_attn_ranges under a fixed KV4_SPLITS); prompts run in one range and always on the wide tiles, also
+// the few rows of a resumed one: an utterance's numbers do not depend on its batch-mates or on how its prompt was cut.
 constexpr int KV4_SPLITS = 16;
 int attn_kv4(fmi_dualar* h, const LayerW& w, int layer, int rows, const int32_t* row_slot, const int32_t* row_pos, hipStream_t s) {
   const Dims& d = h->slow;
@@ -386,9 +386,9 @@ int attn_kv4(fmi_dualar* h, const LayerW& w, int layer, int rows, const int32_t*
   a.max_kv = h->max_seq; a.H = d.H; a.scale = 1.0f / sqrtf((float)d.D);
   if (row_pos) {
     a.q_start = h->kv4_seq; a.kv_len = h->kv4_seq + h->max_batch + 1; a.seq_slot = h->kv4_seq + 2 * h->max_batch + 1;
-    a.n_seqs = h->kv4_n; a.max_q = h->kv4_max_q; a.splits = 1;
+    a.n_seqs = h->kv4_n; a.max_q = h->kv4_max_q; a.splits = 1; a.form = 2;
   } else {
-    a.seq_slot = row_slot; a.n_seqs = rows; a.max_q = 1; a.splits = KV4_SPLITS; a.part = h->kv4_part;
+    a.seq_slot = row_slot; a.n_seqs = rows; a.max_q = 1; a.splits = KV4_SPLITS; a.form = 1; a.part = h->kv4_part;
   }
   FMI_CHECK(launch_kv4_attn(a, s));
   h->launches += a.splits > 1 ? 3 : 2;

@@ -277,19 +277,10 @@ int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s) {
 // =====================================================================================
 //
 // out[row][head] = sum_key softmax_key(scale * q . k) v over the keys [0, pos(row)] of the row's sequence; a row
-// without keys gives 0.  A work-group of 4 waves owns a tile of 16 query columns of one sequence and kv head -- column =
-// (query row, head of the kv head's group), so K and V are read once for all of them -- and one of up to `splits` ranges
-// of 32-key blocks; wave w takes blocks w, w + 4, ... of the range.  Per block:
-//   scores   S^T = K Q^T, v_mfma_f32_16x16x32_bf16: lane (c, g) holds the D / 4 dims from g D / 4 of key c, which is one
-//            consecutive piece of the page and one scale; Q is read in the same order, so no dim is moved;
-//   softmax  fp32, online, per column; the probabilities stay in registers as the B operand of the next product, split
-//            into bf16 high and low parts (two products: 16 significant bits of weight);
-//   output   O^T += V^T P: V is unpacked to bf16 into the wave's LDS rows and read back transposed by
-//            ds_read_b64_tr_b16 (4 keys of one dim per lane).
-// The waves' (m, l, O) are merged through LDS in wave order; with splits > 1 the merged state goes to `part` and
-// kv4_attn_merge_kernel joins the ranges in order.  Keys that a column may not see enter neither the maximum nor the
-// sum nor, where their V is NaN, the product: such blocks are read as 0 and the columns that do see them are set to NaN
-// at the end.
+// without keys gives 0.  Query columns -- column = (query row, head of the kv head's group), so K and V are read once for
+// all heads of a group -- are cut into tiles; a work-group owns a tile and one of up to `splits` ranges of its keys.
+// Keys that a column may not see enter neither the maximum nor the sum nor, where their V is NaN, the product: such blocks
+// are read as 0 and the columns that do see them are set to NaN at the end.
 struct Kv4Span {       // one sequence's query rows and keys, clamped to what the buffers hold
   int slot, row0, nq, kv, cached;
 };
@@ -304,18 +295,57 @@ __device__ inline Kv4Span kv4_span(const Kv4AttnArgs& a, int s) {
   return r;
 }
 
-// the ranges a tile of nb key blocks really uses, at least 8 blocks (256 keys) each: a function of the tile alone.  One
-// range: its work-group writes the output itself and the merge passes the tile's rows by.
-__device__ inline int kv4_attn_ranges(int nb, int splits) { return max(1, min(splits, nb / 8)); }
-// key blocks of 32 that the tile of 16 columns from col0 sees
-__device__ inline int kv4_tile_blocks(const Kv4Span& sp, int G, int col0) {
-  const int nk = min(sp.kv - sp.nq + min(col0 + 15, sp.nq * G - 1) / G + 1, sp.cached);
-  return nk > 0 ? (nk + 31) / 32 : 0;
+// pages of 64 keys that the tile of `tile_cols` columns from col0 sees
+__device__ inline int kv4_tile_pages(const Kv4Span& sp, int G, int col0, int tile_cols) {
+  const int nk = min(sp.kv - sp.nq + min(col0 + tile_cols - 1, sp.nq * G - 1) / G + 1, sp.cached);
+  return nk > 0 ? (nk + KV_PAGE - 1) / KV_PAGE : 0;
+}
+// the ranges a tile of np pages really uses, at least KV4_MIN_PAGES each (one block per wave of a narrow tile): a function of
+// the tile alone.  One range: its work-group writes the output itself and the merge passes the tile's rows by.
+constexpr int KV4_MIN_PAGES = 4;
+__device__ inline int kv4_attn_ranges(const Kv4AttnArgs& a, int np) { return max(1, min(a.splits, np / KV4_MIN_PAGES)); }
+
+// partial states of the key ranges: (m, l) pairs [splits][total_q * H][2], then O [splits][total_q * H][D]
+__device__ inline float* kv4_part_ml(const Kv4AttnArgs& a, int z, int64_t idx) {
+  return a.part + ((int64_t)z * a.total_q * a.H + idx) * 2;
+}
+template <int D>
+__device__ inline float* kv4_part_o(const Kv4AttnArgs& a, int z, int64_t idx) {
+  const int64_t n = (int64_t)a.total_q * a.H;
+  return a.part + (a.splits * n * 2 + 3) / 4 * 4 + (z * n + idx) * D;
 }
 
-template <int D>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
-  constexpr int KB = 32, NW = 4, BLK = kv4_block_bytes(D), NB = D / 32;
+// max / sum over lanes l, l ^ 32 and over l, l ^ 16 inside the VALU
+__device__ inline float max_swap32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float max_swap16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ inline float sum_swap32(float v) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ inline float sum_swap16(float v) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// ---- few query columns: tiles of 16, the kernel of single tokens.  NW waves; wave w takes the 32-key blocks w, w + NW, ...
+// of the range.  Per block:
+//   scores   S^T = K Q^T, v_mfma_f32_16x16x32_bf16: lane (c, g) holds the D / 4 dims from g D / 4 of key c, which is one
+//            consecutive piece of the page and one scale; Q is read in the same order, so no dim is moved;
+//   softmax  fp32, online, per column; the probabilities stay in registers as the B operand of the next product, split
+//            into bf16 high and low parts (two products: 16 significant bits of weight);
+//   output   O^T += V^T P: V is unpacked to bf16 into the wave's LDS rows and read back transposed by
+//            ds_read_b64_tr_b16 (4 keys of one dim per lane).
+// The next block's codes are in flight during a block's arithmetic.  The waves' (m, l, O) are merged through LDS in wave
+// order.
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
+  constexpr int KB = 32, NT = 64 * NW, BLK = kv4_block_bytes(D), NB = D / 32;
   constexpr int KS = D / 32;                     // k-steps of a score product
   constexpr int VROW = D * 2 + 32;               // bytes of a key's row in LDS: 32 more, so that the 4 rows a 16-lane
                                                  // group reads together lie in different banks
@@ -326,20 +356,52 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
   __shared__ int s_nan[NW][NB];
   static_assert(KB * VROW >= 16 * D * 4, "the merge keeps a wave's 16 x D fp32 sums where its V rows were");
 
-  const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 15, g = lane >> 4;
   const int KVH = a.c.KVH, G = a.H / KVH;
   const int tile = blockIdx.x / KVH, kvh = blockIdx.x % KVH, z = blockIdx.y;
   const Kv4Span sp = kv4_span(a, blockIdx.z);
   const int cols = sp.nq * G, col0 = tile * 16;
   if (col0 >= cols) return;
   const int pos0 = sp.kv - sp.nq;                // position of the sequence's first query row (negative: sees nothing)
-  const int col = min(col0 + c, cols - 1);
-  const int qrow = sp.row0 + col / G, head = kvh * G + col % G, qpos = pos0 + col / G;
-  const int vis = min(qpos + 1, sp.cached);      // keys [0, vis) are this column's
-  const int nb = kv4_tile_blocks(sp, G, col0), nz = kv4_attn_ranges(nb, a.splits);
+  const int np = kv4_tile_pages(sp, G, col0, 16), nz = kv4_attn_ranges(a, np);
   if (z >= nz) return;
-  const int b_lo = (int)((int64_t)z * nb / nz), b_hi = (int)((int64_t)(z + 1) * nb / nz);
+  const int col = min(col0 + c, cols - 1);
+  const int qrow = sp.row0 + col / G, head = kvh * G + col % G;
+  const int vis = min(pos0 + col / G + 1, sp.cached);          // keys [0, vis) are this column's
+  const int all_see = min(pos0 + col0 / G + 1, sp.cached);     // keys that every column of the tile sees
+  const int b_lo = (int)((int64_t)z * np / nz) * 2, b_hi = (int)((int64_t)(z + 1) * np / nz) * 2;
   const int32_t* bt = a.c.block_table + (int64_t)sp.slot * a.c.max_pages;
+
+  // K and V codes and scales of one block; a missing page reads page 0 and is skipped later
+  u32x4 vcode[VPASS];
+  uint32_t kcode[2][KS], kscale[2], vscale[VPASS];
+  auto fetch = [&](int kb, int page) {
+    const int pg = page >= 0 && page < a.c.n_pages ? page : 0;
+    const uint8_t* kblk = a.c.pool + ((int64_t)pg * KVH + kvh) * 2 * BLK;
+    const int tok0 = (kb * KB) % KV_PAGE;
+#pragma unroll
+    for (int kt = 0; kt < 2; ++kt) {
+      const int tok = tok0 + kt * 16 + c;
+      const uint8_t* kp = kblk + tok * (D / 2) + g * (D / 8);
+      if constexpr (D == 128) *reinterpret_cast<u32x4*>(kcode[kt]) = *reinterpret_cast<const u32x4*>(kp);
+      else if constexpr (D == 64) *reinterpret_cast<uint2*>(kcode[kt]) = *reinterpret_cast<const uint2*>(kp);
+      else kcode[kt][0] = *reinterpret_cast<const uint32_t*>(kp);
+      kscale[kt] = kblk[KV_PAGE * (D / 2) + tok * NB + g * NB / 4];
+    }
+    const uint8_t* vblk = kblk + BLK;
+#pragma unroll
+    for (int it = 0; it < VPASS; ++it) {
+      const int tok = tok0 + (VP <= KB ? it * VP + lane / VL : min(lane, KB - 1)), part = lane % VL;
+      vcode[it] = *reinterpret_cast<const u32x4*>(vblk + tok * (D / 2) + part * 16);
+      vscale[it] = vblk[KV_PAGE * (D / 2) + tok * NB + part];
+    }
+  };
+  auto page_of = [&](int kb) { return kb < b_hi ? bt[kb >> 1] : -1; };
+
+  int kb = b_lo + wave;
+  int page = page_of(kb);
+  if (kb < b_hi) fetch(kb, page);
+  int next_page = page_of(kb + NW);
 
   bf16x8 qf[KS];                                 // B operand: column c, dims g D / 4 + 8 kk ..
   {
@@ -350,113 +412,121 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
   f32x4 o[D / 16];
 #pragma unroll
   for (int dt = 0; dt < D / 16; ++dt) o[dt] = (f32x4){0.f, 0.f, 0.f, 0.f};
-  float m = -FLT_MAX, l = 0.f;
+  float m = -FLT_MAX, l = 0.f;                   // l: this lane's keys only, joined after the loop
   int nan_key[NB];                               // first key whose V block is NaN, per 32-dim block
 #pragma unroll
   for (int i = 0; i < NB; ++i) nan_key[i] = INT32_MAX;
   const float sl = a.scale * 1.4426950408889634f;   // scores in units of log2
   unsigned char* sv = s_v[wave];
+  const unsigned char* vr = sv + (g * 4 + (c >> 2)) * VROW + (c & 3) * 8;
 
-  for (int kb = b_lo + wave; kb < b_hi; kb += NW) {
-    const int page = bt[(kb * KB) / KV_PAGE];
-    if (page < 0 || page >= a.c.n_pages) continue;         // no page: its keys are masked
-    const int tok0 = (kb * KB) % KV_PAGE;
-    const uint8_t* kblk = a.c.pool + ((int64_t)page * KVH + kvh) * 2 * BLK;
-    const uint8_t* vblk = kblk + BLK;
-    // ---- scores
-    f32x4 sacc[2];
+  for (; kb < b_hi; kb += NW) {
+    const bool there = page >= 0 && page < a.c.n_pages;
+    if (there) {
+      // ---- scores
+      f32x4 sacc[2];
 #pragma unroll
-    for (int kt = 0; kt < 2; ++kt) {
-      const int tok = tok0 + kt * 16 + c;
-      const float ks = kv4_scale(kblk[KV_PAGE * (D / 2) + tok * NB + g * NB / 4]);
-      uint32_t kw[KS];
-      const uint8_t* kp = kblk + tok * (D / 2) + g * (D / 8);
-      if (D == 128) *reinterpret_cast<u32x4*>(kw) = *reinterpret_cast<const u32x4*>(kp);
-      else if (D == 64) *reinterpret_cast<uint2*>(kw) = *reinterpret_cast<const uint2*>(kp);
-      else kw[0] = *reinterpret_cast<const uint32_t*>(kp);
-      sacc[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
+      for (int kt = 0; kt < 2; ++kt) {
+        const float ks = kv4_scale(kscale[kt]);
+        sacc[kt] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int kk = 0; kk < KS; ++kk) {
-        u32x4 kf = kv4_unpack8(kw[kk], ks);
-        sacc[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&kf), qf[kk], sacc[kt], 0, 0, 0);
+        for (int kk = 0; kk < KS; ++kk) {
+          u32x4 kf = kv4_unpack8(kcode[kt][kk], ks);
+          sacc[kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(*reinterpret_cast<bf16x8*>(&kf), qf[kk], sacc[kt], 0, 0, 0);
+        }
       }
-    }
-    // ---- V -> bf16 rows in LDS; rows past the sequence's keys hold whatever was there before: read as 0
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-    __builtin_amdgcn_wave_barrier();             // the previous block's reads are done (same wave)
+      // ---- V -> bf16 rows in LDS; rows past the sequence's keys hold whatever was there before: read as 0
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+      __builtin_amdgcn_wave_barrier();             // the previous block's reads are done (same wave)
+      const bool whole = kb * KB + KB <= sp.cached;
 #pragma unroll
-    for (int it = 0; it < VPASS; ++it) {
-      const int key = it * VP + lane / VL, part = lane % VL;
-      if (VP <= KB || key < KB) {
-        const int tok = tok0 + key, kabs = kb * KB + key;
-        u32x4 vw = *reinterpret_cast<const u32x4*>(vblk + tok * (D / 2) + part * 16);
-        uint32_t b = vblk[KV_PAGE * (D / 2) + tok * NB + part];
-        const bool use = kabs < sp.cached, bad = use && b == KV4_NAN_SCALE;
-        if (__builtin_amdgcn_ballot_w64(bad)) {
+      for (int it = 0; it < VPASS; ++it) {
+        const int key = it * VP + lane / VL, part = lane % VL;
+        if (VP <= KB || key < KB) {
+          const bool use = whole || kb * KB + key < sp.cached, bad = use && vscale[it] == KV4_NAN_SCALE;
+          if (__builtin_amdgcn_ballot_w64(bad)) {
 #pragma unroll
-          for (int i = 0; i < NB; ++i) {
-            const uint64_t hit = __builtin_amdgcn_ballot_w64(bad && part == i);
-            if (hit) nan_key[i] = min(nan_key[i], kb * KB + it * VP + (int)__builtin_ctzll(hit) / VL);
+            for (int i = 0; i < NB; ++i) {
+              const uint64_t hit = __builtin_amdgcn_ballot_w64(bad && part == i);
+              if (hit) nan_key[i] = min(nan_key[i], kb * KB + it * VP + (int)__builtin_ctzll(hit) / VL);
+            }
           }
-        }
-        if (!use || bad) {
-          vw = (u32x4){0, 0, 0, 0};
-          b = 127;
-        }
-        const float vs = kv4_scale(b);
+          if (!use || bad) {
+            vcode[it] = (u32x4){0, 0, 0, 0};
+            vscale[it] = 127;
+          }
+          const float vs = kv4_scale(vscale[it]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          *reinterpret_cast<u32x4*>(sv + key * VROW + part * 64 + i * 16) = kv4_unpack8(vw[i], vs);
+          for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<u32x4*>(sv + key * VROW + part * 64 + i * 16) = kv4_unpack8(vcode[it][i], vs);
+        }
       }
-    }
-    // ---- softmax: lane (c, g) holds keys kt * 16 + g * 4 + j of column c
-    float t[8], mx = -FLT_MAX;
-    bool see[8];
+      const int kb_cur = kb;
+      if (kb + NW < b_hi) fetch(kb + NW, next_page);
+      // ---- softmax: lane (c, g) holds keys kt * 16 + g * 4 + j of column c
+      float t[8], mx = -FLT_MAX;
+      const bool full = kb_cur * KB + KB <= all_see;
+      if (full) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      see[i] = kb * KB + (i >> 2) * 16 + g * 4 + (i & 3) < vis;
-      t[i] = sacc[i >> 2][i & 3] * sl;
-      if (see[i]) mx = fmaxf(mx, t[i]);
-    }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
-    float ps = 0.f;
+        for (int i = 0; i < 8; ++i) {
+          t[i] = sacc[i >> 2][i & 3] * sl;
+          mx = fmaxf(mx, t[i]);
+        }
+      } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      t[i] = see[i] ? __builtin_amdgcn_exp2f(t[i] - mn) : 0.f;
-      ps += t[i];
-    }
-    ps += __shfl_xor(ps, 16, 64);
-    ps += __shfl_xor(ps, 32, 64);
-    l = l * corr + ps;
-    m = mn;
-    u32x4 ph, pl;
+        for (int i = 0; i < 8; ++i) {
+          t[i] = sacc[i >> 2][i & 3] * sl;
+          if (kb_cur * KB + (i >> 2) * 16 + g * 4 + (i & 3) < vis) mx = fmaxf(mx, t[i]);
+        }
+      }
+      mx = max_swap32(max_swap16(mx));
+      const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
+      float ps = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      ph[i] = kv4_pk_bf16(t[2 * i], t[2 * i + 1]);
-      pl[i] = kv4_pk_bf16(t[2 * i] - bf_lo(ph[i]), t[2 * i + 1] - bf_hi(ph[i]));
-    }
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
-    __builtin_amdgcn_wave_barrier();             // this wave's V rows are complete
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
-    // ---- O^T += V^T P: lanes 4 r .. 4 r + 3 of a 16-lane group name row (key) r, lane i gets column (dim) i of the 4
-    const unsigned char* vr = sv + (g * 4 + (c >> 2)) * VROW + (c & 3) * 8;
+      for (int i = 0; i < 8; ++i) {
+        const bool see = full || kb_cur * KB + (i >> 2) * 16 + g * 4 + (i & 3) < vis;
+        t[i] = see ? __builtin_amdgcn_exp2f(t[i] - mn) : 0.f;
+        ps += t[i];
+      }
+      l = l * corr + ps;
+      m = mn;
+      u32x4 ph, pl;
 #pragma unroll
-    for (int dt = 0; dt < D / 16; ++dt) {
-      const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + dt * 32));
-      const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + 16 * VROW + dt * 32));
-      const bf16x8 vf = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+      for (int i = 0; i < 4; ++i) {
+        ph[i] = kv4_pk_bf16(t[2 * i], t[2 * i + 1]);
+        pl[i] = kv4_pk_bf16(t[2 * i] - bf_lo(ph[i]), t[2 * i + 1] - bf_hi(ph[i]));
+      }
+      if (__builtin_amdgcn_ballot_w64(corr != 1.f)) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[dt][j] *= corr;
-      o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, *reinterpret_cast<bf16x8*>(&ph), o[dt], 0, 0, 0);
-      o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, *reinterpret_cast<bf16x8*>(&pl), o[dt], 0, 0, 0);
+        for (int dt = 0; dt < D / 16; ++dt)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[dt][j] *= corr;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+      __builtin_amdgcn_wave_barrier();             // this wave's V rows are complete
+      __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+      // ---- O^T += V^T P: lanes 4 r .. 4 r + 3 of a 16-lane group name row (key) r, lane i gets column (dim) i of the 4
+#pragma unroll
+      for (int dt = 0; dt < D / 16; ++dt) {
+        const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + dt * 32));
+        const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + 16 * VROW + dt * 32));
+        const bf16x8 vf = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, *reinterpret_cast<bf16x8*>(&ph), o[dt], 0, 0, 0);
+        o[dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(vf, *reinterpret_cast<bf16x8*>(&pl), o[dt], 0, 0, 0);
+      }
+    } else if (kb + NW < b_hi) {
+      fetch(kb + NW, next_page);
     }
+    page = next_page;
+    next_page = page_of(kb + 2 * NW);
   }
 
-  // ---- merge the four waves in wave order
+  // ---- merge the waves in wave order
+  l = sum_swap32(sum_swap16(l));
+  const int ncol = min(16, cols - col0);
   __syncthreads();
-  float* s_o = reinterpret_cast<float*>(&s_v[0][0]);       // [NW][16][D]
+  float* s_o = reinterpret_cast<float*>(&s_v[0][0]);       // NW rows of 16 x D sums, KB * VROW bytes apart
+  constexpr int SO = KB * VROW / 4;
   if (g == 0) {
     s_m[wave][c] = m;
     s_l[wave][c] = l;
@@ -464,15 +534,13 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
   if (lane == 0)
 #pragma unroll
     for (int i = 0; i < NB; ++i) s_nan[wave][i] = nan_key[i];
-  float* so = s_o + wave * 16 * D;
+  if (c < ncol) {
 #pragma unroll
-  for (int dt = 0; dt < D / 16; ++dt)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) so[c * D + dt * 16 + g * 4 + j] = o[dt][j];
+    for (int dt = 0; dt < D / 16; ++dt) *reinterpret_cast<f32x4*>(s_o + wave * SO + c * D + dt * 16 + g * 4) = o[dt];
+  }
   __syncthreads();
-  for (int i = tid; i < 16 * D; i += 256) {
+  for (int i = tid; i < ncol * D; i += NT) {
     const int cc = i / D, d = i % D;
-    if (col0 + cc >= cols) continue;
     const int row = (col0 + cc) / G, hd = kvh * G + (col0 + cc) % G;
     float M = -FLT_MAX;
 #pragma unroll
@@ -483,65 +551,374 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
     for (int w = 0; w < NW; ++w) {
       const float wgt = __builtin_amdgcn_exp2f(s_m[w][cc] - M);
       L += s_l[w][cc] * wgt;
-      O += s_o[(w * 16 + cc) * D + d] * wgt;
+      O += s_o[w * SO + cc * D + d] * wgt;
       bad = min(bad, s_nan[w][d / 32]);
     }
-    const int v = min(pos0 + row + 1, sp.cached);
-    if (bad < v) O = __uint_as_float(0x7fc00000u);
-    const int64_t idx = (int64_t)(sp.row0 + row) * a.H + hd;
+    if (bad < min(pos0 + row + 1, sp.cached)) O = __uint_as_float(0x7fc00000u);
     if (nz == 1) {
       a.out[(sp.row0 + row) * a.out_stride + (int64_t)hd * D + d] = L != 0.f ? f2bf(O / L) : (bf16_t)0;
     } else {
-      float* part = a.part + ((int64_t)z * a.total_q * a.H + idx) * (D + 2);
-      part[2 + d] = O;
+      const int64_t idx = (int64_t)(sp.row0 + row) * a.H + hd;
+      kv4_part_o<D>(a, z, idx)[d] = O;
       if (d == 0) {
-        part[0] = M;
-        part[1] = L;
+        kv4_part_ml(a, z, idx)[0] = M;
+        kv4_part_ml(a, z, idx)[1] = L;
       }
     }
   }
 }
 
-// joins the key ranges of one query row and head, in range order.  grid (max_q * H / 2, n_seqs), a wave per (row, head)
-template <int D>
-__global__ __launch_bounds__(128) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
-  const int lane = threadIdx.x & 63;
-  const Kv4Span sp = kv4_span(a, blockIdx.y);
-  const int i = blockIdx.x * 2 + (threadIdx.x >> 6);
-  const int row = i / a.H, hd = i % a.H;
-  if (row >= sp.nq) return;
-  const int G = a.H / a.c.KVH;
-  const int nz = kv4_attn_ranges(kv4_tile_blocks(sp, G, (row * G + hd % G) & ~15), a.splits);
-  if (nz == 1) return;
-  const int64_t step = (int64_t)a.total_q * a.H * (D + 2);
-  const float* part = a.part + ((int64_t)(sp.row0 + row) * a.H + hd) * (D + 2);
-  float M = -FLT_MAX;
-  for (int z = 0; z < nz; ++z) M = fmaxf(M, part[z * step]);
-  float L = 0.f, O[D > 64 ? 2 : 1] = {};
-  for (int z = 0; z < nz; ++z) {
-    const float wgt = __builtin_amdgcn_exp2f(part[z * step] - M);
-    L += part[z * step + 1] * wgt;
-#pragma unroll
-    for (int k = 0; k < (D > 64 ? 2 : 1); ++k)
-      if (k * 64 + lane < D) O[k] += part[z * step + 2 + k * 64 + lane] * wgt;
-  }
-  bf16_t* out = a.out + (sp.row0 + row) * a.out_stride + (int64_t)hd * D;
-#pragma unroll
-  for (int k = 0; k < (D > 64 ? 2 : 1); ++k)
-    if (k * 64 + lane < D) out[k * 64 + lane] = L != 0.f ? f2bf(O[k] / L) : (bf16_t)0;
+// ---- many query columns: tiles of 32 NW = 128, the kernel of prompts.  NW waves of 32 columns each share the pages of 64 keys,
+// staged once per work-group: K unpacked to bf16 and V to fp16 rows in LDS, two buffers and one barrier per page, the next
+// page's codes in flight during a page's arithmetic.  Per page and wave:
+//   scores   S^T = K Q^T, v_mfma_f32_32x32x16_bf16, Q in registers for the whole kernel;
+//   softmax  as above; the probabilities are rounded to fp16 (11 bits: with bf16's 8 a second product with the remainder
+//            would be needed, half as much matrix work again) and stay in registers;
+//   output   O^T += V^T P, v_mfma_f32_32x32x16_f16, V^T by ds_read_b64_tr_b16.
+// V is kept in fp16 relative to 2^E, E = the largest block power among the pages so far (a page's 64 x D / 32 scale bytes are
+// one dword load and a maximum per wave): values are exact down to 2^-23 of the largest block's power, and what falls below
+// is under 2^-24 of the largest value, the size of the rounding of the fp32 sums.  When E grows, O is scaled down like
+// with a growing maximum.
+// The native product of 4-bit K with Q in two 8-bit parts needs no unpacking and the same matrix time, but its sums came out
+// 9e-5 of the absolute sum away from the exact ones (bf16 products: 1e-7), too coarse for scores.
+typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+
+__device__ inline u32x4 kv4_unpack8_f16(uint32_t codes, float scale) {
+  u32x4 r;
+  r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 0));
+  r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 1));
+  r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 2));
+  r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(codes, scale, 3));
+  return r;
+}
+__device__ inline uint32_t kv4_pk_f16(float lo, float hi) {
+  const f32x2_t v = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2_t));
 }
 
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a) {
+  constexpr int NT = 64 * NW, BLK = kv4_block_bytes(D), NB = D / 32, TC = 32 * NW;
+  constexpr int KROW = D * 2 + 16, VROW = D * 2 + 32;      // padded LDS rows: neighbouring keys in different banks
+  constexpr int PIECES = 2 * KV_PAGE * NB;                  // 16-byte pieces (32 codes) of K and V of a page
+  constexpr int PPT = (PIECES + NT - 1) / NT;
+  __shared__ __attribute__((aligned(16))) unsigned char s_k[2][KV_PAGE * KROW];
+  __shared__ __attribute__((aligned(16))) unsigned char s_v[2][KV_PAGE * VROW];
+  __shared__ int s_nan[NB];
+
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31, h = lane >> 5;
+  const int KVH = a.c.KVH, G = a.H / KVH;
+  const int kvh = blockIdx.x % KVH, z = blockIdx.y;
+  const Kv4Span sp = kv4_span(a, blockIdx.z);
+  const int cols = sp.nq * G, tiles = (cols + TC - 1) / TC;
+  const int tile = tiles - 1 - (int)(blockIdx.x / KVH);    // the tiles with the most keys first
+  if (tile < 0) return;
+  const int col0 = tile * TC, pos0 = sp.kv - sp.nq;
+  const int np = kv4_tile_pages(sp, G, col0, TC), nz = kv4_attn_ranges(a, np);
+  if (z >= nz) return;
+  const int p_lo = (int)((int64_t)z * np / nz), p_hi = (int)((int64_t)(z + 1) * np / nz);
+  const int wcol = col0 + 32 * wave;                        // this wave's first column
+  const int col = min(wcol + c, cols - 1);
+  const int qrow = sp.row0 + col / G, head = kvh * G + col % G;
+  const int vis = min(pos0 + col / G + 1, sp.cached);       // keys [0, vis) are this column's
+  // keys that all / any of the wave's columns see (a wave behind the last column sees none)
+  const int all_see = min(pos0 + min(wcol, cols - 1) / G + 1, sp.cached);
+  const int any_see = wcol < cols ? min(pos0 + min(wcol + 31, cols - 1) / G + 1, sp.cached) : 0;
+  const int32_t* bt = a.c.block_table + (int64_t)sp.slot * a.c.max_pages;
+
+  if (tid < NB) s_nan[tid] = INT32_MAX;
+  bf16x8 qf[D / 16];
+  {
+    const bf16_t* qp = a.q + qrow * a.q_stride + (int64_t)head * D + h * 8;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(qp + kk * 16);
+  }
+  f32x16 o[NB];
+#pragma unroll
+  for (int dt = 0; dt < NB; ++dt)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
+  float m = -FLT_MAX, l = 0.f;
+  int E = KV4_MIN_SCALE;
+  const float sl = a.scale * 1.4426950408889634f;
+
+  u32x4 code[PPT];
+  uint32_t scale[PPT], vtok = 0;                            // vtok: the V scales of token `lane`
+  auto fetch = [&](int pg, int page) {
+    const int p = page >= 0 && page < a.c.n_pages ? page : 0;
+    const uint8_t* blk = a.c.pool + ((int64_t)p * KVH + kvh) * 2 * BLK;
+#pragma unroll
+    for (int i = 0; i < PPT; ++i) {
+      const int pc = min(tid + i * NT, PIECES - 1), isv = pc >= PIECES / 2, j = pc % (PIECES / 2);
+      code[i] = *reinterpret_cast<const u32x4*>(blk + isv * BLK + j * 16);
+      scale[i] = blk[isv * BLK + KV_PAGE * (D / 2) + j];
+    }
+    const uint8_t* vs = blk + BLK + KV_PAGE * (D / 2) + lane * NB;
+    if constexpr (NB == 4) vtok = *reinterpret_cast<const uint32_t*>(vs);
+    else if constexpr (NB == 2) vtok = *reinterpret_cast<const uint16_t*>(vs);
+    else vtok = *vs;
+  };
+
+  int pg = p_lo, page = pg < p_hi ? bt[pg] : -1, next_page = pg + 1 < p_hi ? bt[pg + 1] : -1;
+  if (pg < p_hi) fetch(pg, page);
+  __syncthreads();                                          // s_nan
+  for (int it = 0; pg < p_hi; ++pg, it ^= 1) {
+    const bool there = page >= 0 && page < a.c.n_pages;
+    const int tok_end = sp.cached - pg * KV_PAGE;           // tokens of the page at or past this are not the sequence's
+    float grow = 1.f;
+    if (there) {
+      // ---- E: the page's largest V block power
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        const uint32_t b = (vtok >> (8 * i)) & 255u;
+        top = max(top, b == KV4_NAN_SCALE ? 0u : b);
+      }
+      const int pe = (int)wave_max_dpp_u(lane < tok_end ? top : 0u);
+      if (pe > E) {
+        grow = kv4_scale((uint32_t)max(127 + E - pe, 0));
+        E = pe;
+      }
+      // ---- stage
+#pragma unroll
+      for (int i = 0; i < PPT; ++i) {
+        const int pc = tid + i * NT, isv = pc >= PIECES / 2, j = pc % (PIECES / 2), key = j / NB, part = j % NB;
+        if (PIECES % NT == 0 || pc < PIECES) {
+          if (!isv) {
+            const float ks = kv4_scale(scale[i]);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              *reinterpret_cast<u32x4*>(&s_k[it][key * KROW + part * 64 + w * 16]) = kv4_unpack8(code[i][w], ks);
+          } else {
+            const bool use = key < tok_end, bad = use && scale[i] == KV4_NAN_SCALE;
+            if (bad) atomicMin(&s_nan[part], pg * KV_PAGE + key);
+            // (2^-31 and below round every value to 0; a masked block must not pass its scale on: 255 gives NaN even for 0)
+            const float vs = kv4_scale(use && !bad ? (uint32_t)max((int)scale[i] - E + 127, 96) : 127u);
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              *reinterpret_cast<u32x4*>(&s_v[it][key * VROW + part * 64 + w * 16]) =
+                  kv4_unpack8_f16(use && !bad ? code[i][w] : 0u, vs);
+          }
+        }
+      }
+    }
+    __syncthreads();      // the page is staged; and every wave is done with the page before the previous one (same buffer)
+    if (pg + 1 < p_hi) fetch(pg + 1, next_page);
+    if (there && pg * KV_PAGE < any_see) {
+      // ---- scores
+      f32x16 sacc[2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sacc[kt][i] = 0.f;
+        const unsigned char* kr = &s_k[it][(kt * 32 + c) * KROW + h * 16];
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk)
+          sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(kr + kk * 32), qf[kk], sacc[kt], 0, 0, 0);
+      }
+      // ---- softmax: register i of tile kt is key kt * 32 + 8 (i / 4) + 4 h + i % 4 of column c
+      float mx = -FLT_MAX;
+      if (pg * KV_PAGE + KV_PAGE > all_see) {
+        const int lim = vis - pg * KV_PAGE - 4 * h;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const bool see = kt * 32 + 8 * (i >> 2) + (i & 3) < lim;
+            // the scaled score of an unseen key is minus infinity whatever its K holds
+            sacc[kt][i] = see ? sacc[kt][i] * sl : -INFINITY;
+            mx = fmaxf(mx, sacc[kt][i]);
+          }
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            sacc[kt][i] *= sl;
+            mx = fmaxf(mx, sacc[kt][i]);
+          }
+      }
+      mx = max_swap32(mx);
+      const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
+      float ps = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          sacc[kt][i] = __builtin_amdgcn_exp2f(sacc[kt][i] - mn);
+          ps += sacc[kt][i];
+        }
+      l = l * corr + ps;
+      m = mn;
+      const float oc = corr * grow;
+      if (__builtin_amdgcn_ballot_w64(oc != 1.f)) {
+#pragma unroll
+        for (int dt = 0; dt < NB; ++dt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[dt][i] *= oc;
+      }
+      // ---- O^T += V^T P, 16 keys per product: slots (h, 0..3) = keys 4 h .., slots (h, 4..7) = keys 8 + 4 h ..
+      u32x4 pf[4];
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) pf[st][i] = kv4_pk_f16(sacc[st >> 1][(st & 1) * 8 + 2 * i], sacc[st >> 1][(st & 1) * 8 + 2 * i + 1]);
+      // lanes 4 r .. 4 r + 3 of a 16-lane group name row (key) r; lane i of the group gets dim i of the 4 rows
+      const unsigned char* vr = &s_v[it][(4 * h + ((lane & 15) >> 2)) * VROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8];
+#pragma unroll
+      for (int st = 0; st < 4; ++st)
+#pragma unroll
+        for (int dt = 0; dt < NB; ++dt) {
+          const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + st * 16 * VROW + dt * 64));
+          const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + (st * 16 + 8) * VROW + dt * 64));
+          const bf16x8 vf = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf), __builtin_bit_cast(f16x8_t, pf[st]), o[dt], 0, 0, 0);
+        }
+    } else if (grow != 1.f) {
+#pragma unroll
+      for (int dt = 0; dt < NB; ++dt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[dt][i] *= grow;
+    }
+    page = next_page;
+    next_page = pg + 2 < p_hi ? bt[pg + 2] : -1;
+  }
+
+  l = sum_swap32(l);
+  __syncthreads();        // s_nan is complete
+  if (wcol + c >= cols) return;
+  // lane (c, h): dims dt * 32 + 8 (i / 4) + 4 h + i % 4 of column c; O is in units of 2^(E - 127)
+  const int64_t idx = (int64_t)qrow * a.H + head;
+  const float inv = nz > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+  for (int dt = 0; dt < NB; ++dt) {
+    const bool bad = s_nan[dt] < vis;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      f32x4 r;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = bad ? __uint_as_float(0x7fc00000u) : ldexpf(o[dt][q * 4 + j] * inv, E - 127);
+      const int d = dt * 32 + q * 8 + h * 4;
+      if (nz == 1)
+        *reinterpret_cast<uint2*>(a.out + qrow * a.out_stride + (int64_t)head * D + d) = make_uint2(kv4_pk_bf16(r[0], r[1]), kv4_pk_bf16(r[2], r[3]));
+      else
+        *reinterpret_cast<f32x4*>(kv4_part_o<D>(a, z, idx) + d) = r;
+    }
+  }
+  if (nz > 1 && h == 0) {
+    kv4_part_ml(a, z, idx)[0] = m;
+    kv4_part_ml(a, z, idx)[1] = l;
+  }
+}
+
+// joins the key ranges of a query row and head: D / 4 lanes per range, WPR waves (1, or 4 for more than 16 ranges) per row
+// and head, the ranges dealt over the groups of D / 4 lanes and their sums joined in group order.  grid (rows and heads of
+// the longest sequence, 4 / WPR to a work-group; n_seqs).  A group's first ranges are requested before the weights are
+// known: the two loads of a range wait for each other no more than once.
+template <int D, int WPR>
+__global__ __launch_bounds__(256) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
+  constexpr int LN = D / 4, NG = 64 * WPR / LN, PRE = WPR == 1 ? 16 / NG : 4;
+  static_assert(KV4_MAX_SPLITS == 256, "one thread per range below");
+  __shared__ float s_w[4][64], s_red[4], s_sum[4];
+  __shared__ f32x4 s_o[WPR == 1 ? 1 : NG][LN];
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), lane = threadIdx.x & 63;
+  const int tid = WPR == 1 ? lane : (int)threadIdx.x;
+  const Kv4Span sp = kv4_span(a, blockIdx.y);
+  const int item = WPR == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
+  const int row = item / a.H, hd = item % a.H;
+  if (row >= sp.nq) return;
+  const int G = a.H / a.c.KVH, col0 = (row * G + hd % G) / a.tile_cols * a.tile_cols;
+  const int nz = kv4_attn_ranges(a, kv4_tile_pages(sp, G, col0, a.tile_cols));
+  if (nz == 1) return;
+  const int64_t idx = (int64_t)(sp.row0 + row) * a.H + hd;
+  const int gr = tid / LN, ln = tid % LN;
+  const float mz = tid < nz ? kv4_part_ml(a, tid, idx)[0] : -FLT_MAX, lz = tid < nz ? kv4_part_ml(a, tid, idx)[1] : 0.f;
+  f32x4 pre[PRE];
+#pragma unroll
+  for (int k = 0; k < PRE; ++k) pre[k] = *reinterpret_cast<const f32x4*>(kv4_part_o<D>(a, min(gr + k * NG, nz - 1), idx) + ln * 4);
+  float M = wave_max(mz);
+  if constexpr (WPR > 1) {
+    if (lane == 0) s_red[wave] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
+  }
+  const float w = __builtin_amdgcn_exp2f(mz - M);
+  s_w[wave][lane] = w;
+  float L = wave_sum(lz * w);
+  if constexpr (WPR > 1) {
+    if (lane == 0) s_sum[wave] = L;
+    __syncthreads();
+    L = (s_sum[0] + s_sum[1]) + (s_sum[2] + s_sum[3]);
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup");
+    __builtin_amdgcn_wave_barrier();               // this wave's weights
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup");
+  }
+  f32x4 O = {0.f, 0.f, 0.f, 0.f};
+  auto add = [&](int zz, f32x4 v) {
+    const float wz = WPR == 1 ? s_w[wave][zz] : s_w[zz >> 6][zz & 63];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) O[j] += v[j] * wz;
+  };
+#pragma unroll
+  for (int k = 0; k < PRE; ++k)
+    if (gr + k * NG < nz) add(gr + k * NG, pre[k]);
+  for (int zz = gr + PRE * NG; zz < nz; zz += NG) add(zz, *reinterpret_cast<const f32x4*>(kv4_part_o<D>(a, zz, idx) + ln * 4));
+  if constexpr (WPR > 1) {
+    s_o[gr][ln] = O;
+    __syncthreads();
+    if (gr != 0) return;
+    for (int k = 1; k < min(NG, nz); ++k) {
+      const f32x4 v = s_o[k][ln];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) O[j] += v[j];
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (LN <= 8) O[j] += xor_lane_f<8>(O[j], lane);
+      if constexpr (LN <= 16) O[j] = sum_swap16(O[j]);
+      O[j] = sum_swap32(O[j]);
+    }
+    if (gr != 0) return;
+  }
+  float r[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) r[j] = L != 0.f ? O[j] / L : 0.f;
+  *reinterpret_cast<uint2*>(a.out + (sp.row0 + row) * a.out_stride + (int64_t)hd * D + ln * 4) =
+      make_uint2(kv4_pk_bf16(r[0], r[1]), kv4_pk_bf16(r[2], r[3]));
+}
+
+// Narrow tiles (16 columns, 8 waves along the keys) or wide ones (128 columns, 4 waves along the columns).  Both take any
+// count; measured on 8 kv heads x 128 dims, 4 query heads each, narrow / wide in us, at 32, 64 and 128 columns:
+// 1 x 4k keys 14 / 17, 15 / 19, 18 / 23; 8 x 4k 25 / 27, 32 / 34, 51 / 42; 32 x 4k 53 / 78, 94 / 94, 174 / 114.
+constexpr int KV4_NARROW_COLS = 64, KV4_NARROW_TILE = 16, KV4_WIDE_TILE = 128;
+static bool kv4_wide(int max_q, int H, int KVH) { return (int64_t)max_q * (H / KVH) > KV4_NARROW_COLS; }
+
+// Enough work-groups to fill the 256 CUs, no more: a range costs its work-group's start and a partial state.
+// Narrow: one work-group per CU (8 x 2k keys: 256 work-groups 11.4 us, 512 13.0); two where ranges of 32 pages remain, for
+// sequences of different lengths (32 ragged x 8k: 48 us for 512, 54 for 256; 32 x 4k: 36 for 512, 32 for 256).
+// Wide: two fit a CU (8 x 4k keys at 128 columns: 49 us for 256 work-groups, 42 for 512, 52 for 1024), with ranges of at
+// least 8 pages where more than 128 rows would write partial states (32 x 500 keys at 128 columns: 24 us in one range, 50 in
+// two of 4 pages; 1 x 4k at 96 columns: 21 us in ranges of 4 pages, 26 in ranges of 8).
 int kv4_attn_splits(int n_seqs, int max_q, int max_kv, int H, int KVH) {
-  const int64_t tiles = (int64_t)n_seqs * KVH * (((int64_t)max_q * (H / KVH) + 15) / 16);
-  const int64_t want = (1024 + tiles - 1) / std::max<int64_t>(tiles, 1), most = std::max(1, max_kv / 256);
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min(want, most), 256));
+  const bool wide = kv4_wide(max_q, H, KVH);
+  const int tc = wide ? KV4_WIDE_TILE : KV4_NARROW_TILE, pages = max_kv / KV_PAGE;
+  const int64_t tiles = std::max<int64_t>(1, (int64_t)n_seqs * KVH * (((int64_t)max_q * (H / KVH) + tc - 1) / tc));
+  int64_t want = (wide ? 512 : 256) / tiles;
+  if (!wide && tiles >= 128 && 512 / tiles * 32 <= pages) want = 512 / tiles;
+  const int least = wide && (int64_t)n_seqs * max_q > 128 ? 8 : KV4_MIN_PAGES;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, pages / least), KV4_MAX_SPLITS));
 }
 
 int64_t kv4_attn_part_floats(int total_q, int H, int D, int splits) {
-  return splits > 1 ? (int64_t)splits * total_q * H * (D + 2) : 0;
+  const int64_t n = (int64_t)total_q * H * splits;
+  return splits > 1 ? (n * 2 + 3) / 4 * 4 + n * D : 0;
 }
 
-int launch_kv4_attn(const Kv4AttnArgs& a, hipStream_t s) {
+int launch_kv4_attn(const Kv4AttnArgs& a_, hipStream_t s) {
+  Kv4AttnArgs a = a_;
   FMI_CHECK(kv4_check_cache(a.c));
   const int D = a.c.D;
   FMI_REQUIRE(a.H >= 1 && a.H % a.c.KVH == 0, "kv4 attention: %d query heads over %d kv heads", a.H, a.c.KVH);
@@ -551,14 +928,20 @@ int launch_kv4_attn(const Kv4AttnArgs& a, hipStream_t s) {
   FMI_CHECK(kv4_check_rows("q", a.q, a.q_stride, a.H, D));
   FMI_CHECK(kv4_check_rows("out", a.out, a.out_stride, a.H, D));
   FMI_REQUIRE(a.seq_slot || a.n_seqs <= a.c.n_slots, "kv4 attention: %d sequences, block table of %d", a.n_seqs, a.c.n_slots);
-  FMI_REQUIRE(a.splits >= 1 && a.splits <= 256 && (a.splits == 1 || a.part), "kv4 attention: bad split of the keys");
-  const int64_t tiles = ((int64_t)a.max_q * (a.H / a.c.KVH) + 15) / 16;
+  FMI_REQUIRE(a.splits >= 1 && a.splits <= KV4_MAX_SPLITS && (a.splits == 1 || a.part), "kv4 attention: bad split of the keys");
+  const int64_t cols = (int64_t)a.max_q * (a.H / a.c.KVH);
+  const bool wide = a.form ? a.form == 2 : kv4_wide(a.max_q, a.H, a.c.KVH);
+  a.tile_cols = wide ? KV4_WIDE_TILE : KV4_NARROW_TILE;
+  const int64_t tiles = (cols + a.tile_cols - 1) / a.tile_cols;
   FMI_REQUIRE(tiles * a.c.KVH < (int64_t)1 << 31 && (int64_t)a.max_q * a.H < (int64_t)1 << 31, "kv4 attention: too many query rows");
-  const dim3 grid((unsigned)(tiles * a.c.KVH), a.splits, a.n_seqs), mgrid((unsigned)(((int64_t)a.max_q * a.H + 1) / 2), a.n_seqs);
-#define FMI_KV4_ATTN(D_)                                                                        \
-  do {                                                                                          \
-    hipLaunchKernelGGL((kv4_attn_kernel<D_>), grid, dim3(256), 0, s, a);                        \
-    if (a.splits > 1) hipLaunchKernelGGL((kv4_attn_merge_kernel<D_>), mgrid, dim3(128), 0, s, a); \
+  const dim3 grid((unsigned)(tiles * a.c.KVH), a.splits, a.n_seqs), 
+             mgrid((unsigned)(((int64_t)a.max_q * a.H + (a.splits > 16 ? 0 : 3)) / (a.splits > 16 ? 1 : 4)), a.n_seqs);
+#define FMI_KV4_ATTN(D_)                                                                                       \
+  do {                                                                                                         \
+    if (wide) hipLaunchKernelGGL((kv4_attn_wide_kernel<D_, KV4_WIDE_TILE / 32>), grid, dim3(2 * KV4_WIDE_TILE), 0, s, a); \
+    else hipLaunchKernelGGL((kv4_attn_kernel<D_, 8>), grid, dim3(512), 0, s, a);                               \
+    if (a.splits > 16) hipLaunchKernelGGL((kv4_attn_merge_kernel<D_, 4>), mgrid, dim3(256), 0, s, a);          \
+    else if (a.splits > 1) hipLaunchKernelGGL((kv4_attn_merge_kernel<D_, 1>), mgrid, dim3(256), 0, s, a);      \
   } while (0)
   if (D == 128) FMI_KV4_ATTN(128);
   else if (D == 64) FMI_KV4_ATTN(64);
@@ -615,7 +998,7 @@ static int kv4_splits_of(const fmi_kv4_cache* cache, const fmi_kv4_query* q) {
 }
 
 int64_t fmi_kv4_attention_ws_bytes(const fmi_kv4_cache* cache, const fmi_kv4_query* q) {
-  if (!cache || !q || cache->n_kv_head < 1 || q->n_head < 1 || q->splits < 0 || q->splits > 256 || q->total_q < 0 ||
+  if (!cache || !q || cache->n_kv_head < 1 || q->n_head < 1 || q->splits < 0 || q->splits > KV4_MAX_SPLITS || q->total_q < 0 ||
       q->max_q < 0 || q->n_seqs < 0 || q->max_kv < 0)
     return set_error(FMI_EINVAL, "kv4 attention: bad sizes");
   return 4 * kv4_attn_part_floats(q->total_q, q->n_head, cache->head_dim, kv4_splits_of(cache, q));

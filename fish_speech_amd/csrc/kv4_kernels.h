@@ -43,6 +43,8 @@ struct Kv4ReadArgs {
 };
 int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s);
 
+constexpr int KV4_MAX_SPLITS = 256;
+
 struct Kv4AttnArgs {
   Kv4Cache c;
   const bf16_t* q;                          // rows of [H][D]
@@ -56,6 +58,8 @@ struct Kv4AttnArgs {
   float scale;
   int splits;                               // most key ranges per query tile (kv4_attn_splits), >= 1
   float* part;                              // splits > 1: kv4_attn_part_floats
+  int form;                                 // 0: the tile width follows max_q; 1 / 2: narrow / wide tiles, whatever max_q is
+  int tile_cols;                            // set by the launch: query columns per tile
 };
 // most key ranges a call of these sizes is split into: a function of the host's sizes only
 int kv4_attn_splits(int n_seqs, int max_q, int max_kv, int H, int KVH);

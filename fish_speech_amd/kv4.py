@@ -8,16 +8,23 @@ captured into a HIP graph; there is no CPU fallback.
 """
 from __future__ import annotations
 
-import ctypes as C
 import math
+import struct
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
-from ._lib import FishmiError, Kv4CacheC, Kv4QueryC, Kv4RowsC, check
+from ._lib import FishmiError, check
 
 PAGE = 64   # tokens per page
+
+# The argument structs of include/fishmi.h as packed bytes.  A generation loop makes one append and one attend per layer and
+# token, each a few microseconds of GPU work: building a ctypes.Structure field by field took longer than the launch.
+_CACHE = struct.Struct("@PPiiiii")              # fmi_kv4_cache
+_ROWS = struct.Struct("@PPPqqqPqiPPdPiiiPPi")   # fmi_kv4_rows
+_QUERY = struct.Struct("@PqiPPiiiifi")          # fmi_kv4_query
+_BF16, _I32 = torch.bfloat16, torch.int32
 
 
 def page_bytes(n_kv_head: int, head_dim: int) -> int:
@@ -34,52 +41,65 @@ class KV4Cache:
     an id outside [0, n_pages) (-1, say) means "no page"."""
 
     def __init__(self, n_pages: int, n_kv_head: int, head_dim: int, device="cuda:0", pool: Optional[torch.Tensor] = None):
-        self.lib = _lib.load()
-        self.device = torch.device(device)
-        if self.device.type != "cuda":
+        device = torch.device(device)
+        if device.type != "cuda":
             raise FishmiError("KV4Cache needs a GPU device (no CPU fallback)")
-        if self.device.index is None:
-            self.device = torch.device("cuda", torch.cuda.current_device())
-        self.n_pages, self.n_kv_head, self.head_dim = int(n_pages), int(n_kv_head), int(head_dim)
-        shape = (self.n_pages, self.n_kv_head, 2, page_bytes(n_kv_head, head_dim) // (2 * self.n_kv_head))
-        if self.n_pages < 1:
+        if device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        block = page_bytes(n_kv_head, head_dim) // (2 * int(n_kv_head))
+        if n_pages < 1:
             raise ValueError(f"n_pages {n_pages} must be positive")
+        shape = (int(n_pages), int(n_kv_head), 2, block)
         if pool is None:
-            pool = torch.zeros(shape, dtype=torch.uint8, device=self.device)
-        elif pool.dtype != torch.uint8 or tuple(pool.shape) != shape or pool.device != self.device or not pool.is_contiguous():
-            raise ValueError(f"pool must be a contiguous uint8 tensor of shape {shape} on {self.device}")
-        self.pool = pool
+            pool = torch.zeros(shape, dtype=torch.uint8, device=device)
+        elif pool.dtype != torch.uint8 or tuple(pool.shape) != shape or pool.device != device or not pool.is_contiguous():
+            raise ValueError(f"pool must be a contiguous uint8 tensor of shape {shape} on {device}")
+        self._setup(pool, int(head_dim))
+
+    def _setup(self, pool: torch.Tensor, head_dim: int):
+        self.lib = _lib.load()
+        self.pool, self.device, self.head_dim = pool, pool.device, head_dim
+        self.n_pages, self.n_kv_head = int(pool.shape[0]), int(pool.shape[1])
+        self._dev = pool.get_device()
 
     # ---- argument checks
-    def _index(self, name: str, t: torch.Tensor, n: Optional[int] = None) -> torch.Tensor:
-        if t.dtype != torch.int32 or t.device != self.device or t.dim() != 1 or not t.is_contiguous():
+    def _index(self, name: str, t: torch.Tensor, n: int) -> int:
+        """-> the address of a contiguous int32 vector of n entries"""
+        if t.dtype is not _I32 or t.get_device() != self._dev or t.dim() != 1 or not t.is_contiguous():
             raise ValueError(f"{name} must be a contiguous 1-d int32 tensor on {self.device}")
-        if n is not None and t.numel() != n:
-            raise ValueError(f"{name} has {t.numel()} entries, expected {n}")
-        return t
+        if t.shape[0] != n:
+            raise ValueError(f"{name} has {t.shape[0]} entries, expected {n}")
+        return t.data_ptr()
 
-    def _rows(self, name: str, t: torch.Tensor, rows: Optional[int] = None, heads: Optional[int] = None) -> torch.Tensor:
-        if t.dtype != torch.bfloat16 or t.device != self.device or t.dim() != 3 or t.shape[2] != self.head_dim:
-            raise ValueError(f"{name} must be a bfloat16 tensor (rows, heads, {self.head_dim}) on {self.device}")
-        if (rows is not None and t.shape[0] != rows) or (heads is not None and t.shape[1] != heads):
-            raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({rows}, {heads}, {self.head_dim})")
-        if t.numel() and (t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != self.head_dim)):
-            raise ValueError(f"{name}: the heads of a row must be contiguous (strides {t.stride()})")
-        return t
+    def _rows(self, name: str, t: torch.Tensor, rows: int, heads: int) -> int:
+        """-> the row stride of a bf16 tensor (rows, heads, head_dim) whose rows are contiguous"""
+        D = self.head_dim
+        if t.dtype is not _BF16 or t.get_device() != self._dev or t.dim() != 3:
+            raise ValueError(f"{name} must be a bfloat16 tensor (rows, heads, {D}) on {self.device}")
+        r, h, d = t.shape
+        if r != rows or h != heads or d != D:
+            raise ValueError(f"{name} has shape {(r, h, d)}, expected {(rows, heads, D)}")
+        s0, s1, s2 = t.stride()
+        if r and (s2 != 1 or (s1 != D and h != 1)):
+            raise ValueError(f"{name}: the heads of a row must be contiguous (strides {(s0, s1, s2)})")
+        return s0 if r > 1 else h * D
 
-    @staticmethod
-    def _stride(t: torch.Tensor) -> int:
-        return int(t.stride(0)) if t.shape[0] > 1 else int(t.shape[1] * t.shape[2])
-
-    def _c(self, block_table: torch.Tensor) -> Kv4CacheC:
-        if (block_table.dtype != torch.int32 or block_table.device != self.device or block_table.dim() != 2
+    def _cache(self, block_table: torch.Tensor) -> bytes:
+        if (block_table.dtype is not _I32 or block_table.get_device() != self._dev or block_table.dim() != 2
                 or not block_table.is_contiguous()):
             raise ValueError(f"block_table must be a contiguous int32 tensor (n_seqs, max_pages) on {self.device}")
-        return Kv4CacheC(self.pool.data_ptr(), block_table.data_ptr(), self.n_pages, self.n_kv_head, self.head_dim,
-                         block_table.shape[0], block_table.shape[1])
+        n, w = block_table.shape
+        return _CACHE.pack(self.pool.data_ptr(), block_table.data_ptr(), self.n_pages, self.n_kv_head, self.head_dim, n, w)
 
-    def _stream(self):
-        return C.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+    def _call(self, fn, *args):
+        """fn(*args, stream) with the cache's device current"""
+        if torch.cuda.current_device() == self._dev:
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(self._dev))
+        else:
+            with torch.cuda.device(self._dev):
+                rc = fn(*args, torch._C._cuda_getCurrentRawStream(self._dev))
+        if rc:
+            check(rc)
 
     # ---- operators
     def append(self, k: torch.Tensor, v: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor,
@@ -95,41 +115,40 @@ class KV4Cache:
 
         Rows whose sequence or position lies outside the block table (or the rotation table) are padding: nothing is
         written for them, in the cache or in ``q_out``.  A (sequence, position) pair may appear once per call."""
-        rows = int(k.shape[0])
-        self._rows("k", k, rows, self.n_kv_head)
-        self._rows("v", v, rows, self.n_kv_head)
-        self._index("row_seq", row_seq, rows)
-        self._index("row_pos", row_pos, rows)
-        a = Kv4RowsC(k_dev=k.data_ptr(), v_dev=v.data_ptr(), k_stride=self._stride(k), v_stride=self._stride(v),
-                     norm_eps=float(eps), row_seq_dev=row_seq.data_ptr(), row_pos_dev=row_pos.data_ptr(), rows=rows)
+        rows, KVH = k.shape[0], self.n_kv_head
+        ks, vs = self._rows("k", k, rows, KVH), self._rows("v", v, rows, KVH)
+        ps, pp = self._index("row_seq", row_seq, rows), self._index("row_pos", row_pos, rows)
         if rope_layout not in ("interleaved", "half"):
             raise ValueError(f"rope_layout {rope_layout!r}: 'interleaved' or 'half'")
-        for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-            if w is not None and (w.dtype != torch.bfloat16 or w.device != self.device or tuple(w.shape) != (self.head_dim,)
-                                  or not w.is_contiguous()):
-                raise ValueError(f"{name} must be a contiguous bfloat16 tensor ({self.head_dim},) on {self.device}")
-        if q is None and (q_norm is not None or q_out is not None):
+        half = rope_layout == "half"
+        qp = qs = op = os = heads = qn = kn = rp = rl = rd = 0
+        if q is not None:
+            heads = q.shape[1] if q.dim() == 3 else 0
+            qs, qp = self._rows("q", q, rows, heads), q.data_ptr()
+            if q_out is None:
+                q_out = torch.empty(rows, heads, self.head_dim, dtype=_BF16, device=self.device)
+            os, op = self._rows("q_out", q_out, rows, heads), q_out.data_ptr()
+        elif q_norm is not None or q_out is not None:
             raise ValueError("q_norm and q_out go with q")
         if rope is not None:
-            if rope.dtype != torch.bfloat16 or rope.device != self.device or rope.dim() != 3 or rope.shape[2] != 2 \
-                    or not rope.is_contiguous():
+            if (rope.dtype is not _BF16 or rope.get_device() != self._dev or rope.dim() != 3 or rope.shape[2] != 2
+                    or not rope.is_contiguous()):
                 raise ValueError(f"rope must be a contiguous bfloat16 tensor (positions, dims / 2, 2) on {self.device}")
-            a.rope_dev, a.rope_len, a.rope_dim = rope.data_ptr(), rope.shape[0], 2 * rope.shape[1]
-            a.rope_half = int(rope_layout == "half")
-        a.q_norm_dev = q_norm.data_ptr() if q_norm is not None else None
-        a.k_norm_dev = k_norm.data_ptr() if k_norm is not None else None
-        if q is not None:
-            self._rows("q", q, rows)
-            if q_out is None:
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-            self._rows("q_out", q_out, rows, int(q.shape[1]))
-            if rope is not None and a.rope_half and q_out.data_ptr() == q.data_ptr() and rows:
+            rp, rl, rd = rope.data_ptr(), rope.shape[0], 2 * rope.shape[1]
+            if half and qp and op == qp:
                 raise ValueError("the half-split rotation cannot write q_out over q")
-            a.q_dev, a.q_stride, a.n_head = q.data_ptr(), self._stride(q), int(q.shape[1])
-            a.q_out_dev, a.q_out_stride = q_out.data_ptr(), self._stride(q_out)
-        with torch.cuda.device(self.device):
-            check(self.lib.fmi_op_kv4_append(C.byref(self._c(block_table)), C.byref(a), self._stream()))
+        if q_norm is not None:
+            qn = self._weight("q_norm", q_norm)
+        if k_norm is not None:
+            kn = self._weight("k_norm", k_norm)
+        a = _ROWS.pack(qp, k.data_ptr(), v.data_ptr(), qs, ks, vs, op, os, heads, qn, kn, eps, rp, rl, rd, half, ps, pp, rows)
+        self._call(self.lib.fmi_op_kv4_append, self._cache(block_table), a)
         return q_out
+
+    def _weight(self, name: str, w: torch.Tensor) -> int:
+        if w.dtype is not _BF16 or w.get_device() != self._dev or tuple(w.shape) != (self.head_dim,) or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous bfloat16 tensor ({self.head_dim},) on {self.device}")
+        return w.data_ptr()
 
     def attend(self, q: torch.Tensor, q_start: torch.Tensor, kv_len: torch.Tensor, block_table: torch.Tensor, *,
                max_q: int, max_kv: int, out: Optional[torch.Tensor] = None, scale: Optional[float] = None,
@@ -139,41 +158,35 @@ class KV4Cache:
         both int32 on the device, so a captured graph replays with new lengths.  ``max_q`` / ``max_kv``: upper bounds of
         one sequence's rows and keys (rows beyond ``max_q`` are not computed; ``max_kv`` only tunes the launch).  Rows
         that see no key give 0.  Rows behind the last sequence are left as they were in ``out`` (undefined without one).
-        ``splits``: key ranges per query tile, 0 = chosen from the sizes; with a fixed number a row's bits do not depend
-        on the other sequences of the call."""
-        self._rows("q", q)
-        n_seqs = int(block_table.shape[0])
-        self._index("q_start", q_start, n_seqs + 1)
-        self._index("kv_len", kv_len, n_seqs)
+        ``splits``: key ranges per query tile, 0 = chosen from the sizes; with a fixed number (and ``max_q``) a row's bits
+        do not depend on the other sequences of the call."""
+        n, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0
+        qs = self._rows("q", q, n, heads)
+        c = self._cache(block_table)
+        n_seqs = block_table.shape[0]
+        sp, lp = self._index("q_start", q_start, n_seqs + 1), self._index("kv_len", kv_len, n_seqs)
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        self._rows("out", out, int(q.shape[0]), int(q.shape[1]))
-        c = self._c(block_table)
-        a = Kv4QueryC(q_dev=q.data_ptr(), q_stride=self._stride(q), n_head=int(q.shape[1]), q_start_dev=q_start.data_ptr(),
-                      kv_len_dev=kv_len.data_ptr(), n_seqs=n_seqs, total_q=int(q.shape[0]), max_q=int(max_q),
-                      max_kv=int(max_kv), scale=1.0 / math.sqrt(self.head_dim) if scale is None else float(scale),
-                      splits=int(splits))
-        need = self.lib.fmi_kv4_attention_ws_bytes(C.byref(c), C.byref(a))
-        if need < 0:
-            check(int(need))
-        # from torch's allocator: ordered with the stream, private to a graph that is being captured
-        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None
-        with torch.cuda.device(self.device):
-            check(self.lib.fmi_op_kv4_attention(C.byref(c), C.byref(a), C.c_void_p(out.data_ptr()), self._stride(out),
-                                                C.c_void_p(ws.data_ptr() if ws is not None else None), need,
-                                                self._stream()))
+            out = torch.empty(n, heads, self.head_dim, dtype=_BF16, device=self.device)
+        os = self._rows("out", out, n, heads)
+        if scale is None:
+            scale = 1.0 / math.sqrt(self.head_dim)
+        a = _QUERY.pack(q.data_ptr(), qs, heads, sp, lp, n_seqs, n, max_q, max_kv, scale, splits)
+        need = self.lib.fmi_kv4_attention_ws_bytes(c, a)
+        ws = None
+        if need > 0:       # from torch's allocator: ordered with the stream, private to a graph that is being captured
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+        elif need < 0:
+            check(need)
+        self._call(self.lib.fmi_op_kv4_attention, c, a, out.data_ptr(), os, ws.data_ptr() if need else 0, need)
         return out
 
     def read(self, row_seq: torch.Tensor, row_pos: torch.Tensor, block_table: torch.Tensor
              ) -> Tuple[torch.Tensor, torch.Tensor]:
         """The stored values of (sequence, position) pairs: k, v bf16 (rows, n_kv_head, head_dim), exact.  Pairs outside
         the sequences, the block table or the pool read as 0."""
-        rows = int(row_seq.numel())
-        self._index("row_seq", row_seq)
-        self._index("row_pos", row_pos, rows)
-        k, v = (torch.empty(rows, self.n_kv_head, self.head_dim, dtype=torch.bfloat16, device=self.device) for _ in range(2))
-        with torch.cuda.device(self.device):
-            check(self.lib.fmi_op_kv4_read(C.byref(self._c(block_table)), C.c_void_p(row_seq.data_ptr()),
-                                           C.c_void_p(row_pos.data_ptr()), rows, C.c_void_p(k.data_ptr()),
-                                           C.c_void_p(v.data_ptr()), self._stream()))
+        rows = row_seq.shape[0] if row_seq.dim() == 1 else -1
+        sp, pp = self._index("row_seq", row_seq, rows), self._index("row_pos", row_pos, rows)
+        k = torch.empty(rows, self.n_kv_head, self.head_dim, dtype=_BF16, device=self.device)
+        v = torch.empty(rows, self.n_kv_head, self.head_dim, dtype=_BF16, device=self.device)
+        self._call(self.lib.fmi_op_kv4_read, self._cache(block_table), sp, pp, rows, k.data_ptr(), v.data_ptr())
         return k, v

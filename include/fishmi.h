@@ -317,7 +317,9 @@ int fmi_op_kv4_read(const fmi_kv4_cache* cache, const int32_t* row_seq_dev, cons
  * scores, softmax and sums, one rounding to bf16.  A row that sees no key gives 0; rows past the last sequence stay as
  * they were.  max_q and max_kv bound the rows and keys of any sequence (they size the launch; rows beyond max_q of a
  * sequence are not computed).  splits: key ranges a query tile is divided into, 1 .. 256, or 0 for a choice made from
- * n_seqs, max_q and max_kv alone; with a fixed value a row's bits do not depend on the other sequences of the call. */
+ * n_seqs, max_q and max_kv alone; with a fixed value (and max_q) a row's bits do not depend on the other sequences of the
+ * call.  Up to 64 query columns (max_q times heads per kv head) the softmax weights enter the product with 16 significant
+ * bits, above that with fp16's 11. */
 typedef struct fmi_kv4_query {
   const void* q_dev;
   int64_t q_stride;

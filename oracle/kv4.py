@@ -74,9 +74,10 @@ def rotate(y: torch.Tensor, cs: Optional[torch.Tensor], half: bool) -> torch.Ten
 
 
 def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, past: int, scale: float,
-           seen: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+           seen: Optional[torch.Tensor] = None, weight: float = 2.0 ** -16) -> Tuple[torch.Tensor, torch.Tensor]:
     """One sequence: q (n, H, D) at positions past .. past + n - 1, k / v (keys, KVH, D) float64; `seen` (keys,) = keys that
-    exist at all.  -> output float64 and, per output, a bound of the arithmetic's error before the last rounding."""
+    exist at all; `weight` = relative rounding of a softmax weight (bf16 high + low part 2^-16, fp16 2^-11).  -> output float64
+    and, per output, a bound of the arithmetic's error before the last rounding."""
     n, H, D = q.shape
     G = H // k.shape[1]
     out = torch.zeros(n, H, D, dtype=torch.float64)
@@ -93,7 +94,8 @@ def attend(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, past: int, scale: 
             p = torch.exp(s - s.max())
             out[i, h] = p @ vv / p.sum()
             # fp32: a score is off by (D + 4) roundings of its absolute products, which moves every weight by that much;
-            # weights carry 2^-16 (bf16 high + low part) and the fp32 exponential; sums of len(idx) terms add a rounding each
+            # weights carry their rounding and the fp32 exponential's 2^-16; sums of len(idx) terms add a rounding each, and a
+            # weight below fp16's smallest step (2^-25 rounds to 0) loses no more than that
             ds = (D + 4) * 2.0 ** -24 * float((kk.abs() @ qq.abs()).max()) * abs(scale)
-            bound[i, h] = (4 * ds + 2.0 ** -15 + idx.numel() * 2.0 ** -24) * float(vv.abs().max())
+            bound[i, h] = (4 * ds + weight + 2.0 ** -16 + idx.numel() * 2.0 ** -24) * float(vv.abs().max())
     return out, bound

@@ -1,13 +1,12 @@
 """The 4-bit K/V cache without a GPU: the number format's oracle, and every refusal of the C entry points and of the Python
 object (all of them are decided on the host before anything is launched)."""
-import ctypes as C
 import math
 
 import pytest
 import torch
 
 from fish_speech_amd import _lib, kv4
-from fish_speech_amd._lib import FishmiError, Kv4CacheC, Kv4QueryC, Kv4RowsC
+from fish_speech_amd._lib import FishmiError
 from oracle import kv4 as O
 
 A = 1 << 20   # an aligned address that is never dereferenced: every call below is refused first
@@ -50,24 +49,46 @@ def test_nonfinite_blocks_read_as_nan_and_leave_their_neighbours():
 # ------------------------------------------------------------------------------------------------ refusals: C ABI
 
 
+def _pack(layout, fields, kw):
+    """The fields in the order of include/fishmi.h -> the packed struct."""
+    assert set(kw) <= set(fields)
+    return layout.pack(*[v or 0 for v in dict(fields, **kw).values()])
+
+
+def test_packed_structs_match_the_header():
+    """Field types and order of the three structs in include/fishmi.h, and their sizes as the C compiler lays them out."""
+    import os
+    import re
+
+    src = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "fishmi.h")).read()
+    src = re.sub(r"/\*.*?\*/", "", src, flags=re.S)
+    kinds = {"int32_t": "i", "int64_t": "q", "float": "f", "double": "d"}
+    for name, layout in (("fmi_kv4_cache", kv4._CACHE), ("fmi_kv4_rows", kv4._ROWS), ("fmi_kv4_query", kv4._QUERY)):
+        body = re.search(r"typedef struct %s \{(.*?)\}" % name, src, flags=re.S).group(1)
+        fmt = "@"
+        for decl in filter(None, (d.strip() for d in body.split(";"))):
+            base = re.sub(r"^const\s+", "", decl).split()[0].rstrip("*")
+            for var in re.sub(r"^(const\s+)?\w+", "", decl).split(","):
+                fmt += "P" if "*" in var else kinds[base]
+        assert fmt == layout.format, name
+
+
 def _cache(**kw):
     d = dict(pool_dev=A, block_table_dev=A, n_pages=4, n_kv_head=2, head_dim=64, n_seqs=3, max_pages=5)
-    d.update(kw)
-    return Kv4CacheC(**d)
+    return _pack(kv4._CACHE, d, kw)
 
 
 def _rows(**kw):
     d = dict(q_dev=A, k_dev=A, v_dev=A, q_stride=256, k_stride=128, v_stride=128, q_out_dev=A, q_out_stride=256, n_head=4,
-             norm_eps=1e-6, rope_dev=A, rope_len=10, rope_dim=64, row_seq_dev=A, row_pos_dev=A, rows=7)
-    d.update(kw)
-    return Kv4RowsC(**d)
+             q_norm_dev=None, k_norm_dev=None, norm_eps=1e-6, rope_dev=A, rope_len=10, rope_dim=64, rope_half=0,
+             row_seq_dev=A, row_pos_dev=A, rows=7)
+    return _pack(kv4._ROWS, d, kw)
 
 
 def _query(**kw):
     d = dict(q_dev=A, q_stride=256, n_head=4, q_start_dev=A, kv_len_dev=A, n_seqs=3, total_q=5, max_q=2, max_kv=100,
              scale=0.1, splits=1)
-    d.update(kw)
-    return Kv4QueryC(**d)
+    return _pack(kv4._QUERY, d, kw)
 
 
 BAD_CACHES = [dict(pool_dev=None), dict(pool_dev=A + 8), dict(block_table_dev=None), dict(block_table_dev=A + 2), dict(head_dim=48),
@@ -78,10 +99,10 @@ BAD_CACHES = [dict(pool_dev=None), dict(pool_dev=A + 8), dict(block_table_dev=No
 @pytest.mark.parametrize("bad", BAD_CACHES, ids=str)
 def test_every_entry_point_refuses_a_bad_cache(bad):
     lib = _lib.load()
-    c = C.byref(_cache(**bad))
-    assert lib.fmi_op_kv4_append(c, C.byref(_rows()), None) == -1
+    c = _cache(**bad)
+    assert lib.fmi_op_kv4_append(c, _rows(), None) == -1
     assert lib.fmi_op_kv4_read(c, A, A, 3, A, A, None) == -1
-    assert lib.fmi_op_kv4_attention(c, C.byref(_query()), A, 256, None, 0, None) == -1
+    assert lib.fmi_op_kv4_attention(c, _query(), A, 256, None, 0, None) == -1
     assert b"kv4" in lib.fmi_last_error()
 
 
@@ -92,7 +113,7 @@ def test_every_entry_point_refuses_a_bad_cache(bad):
     dict(rope_dim=80), dict(rope_len=0), dict(rope_dev=A + 4), dict(q_norm_dev=A + 2), dict(k_norm_dev=A + 8),
     dict(q_dev=None, q_norm_dev=A)], ids=str)
 def test_append_refusals(bad):
-    assert _lib.load().fmi_op_kv4_append(C.byref(_cache()), C.byref(_rows(**bad)), None) == -1
+    assert _lib.load().fmi_op_kv4_append(_cache(), _rows(**bad), None) == -1
 
 
 @pytest.mark.parametrize("bad", [
@@ -101,13 +122,13 @@ def test_append_refusals(bad):
     dict(splits=-1), dict(splits=257)], ids=str)
 def test_attention_refusals(bad):
     lib = _lib.load()
-    c, q = C.byref(_cache()), C.byref(_query(**bad))
+    c, q = _cache(), _query(**bad)
     assert lib.fmi_op_kv4_attention(c, q, A, 256, A, 1 << 30, None) == -1
 
 
 def test_attention_refuses_a_missing_or_small_workspace_and_bad_outputs():
     lib = _lib.load()
-    c, q = C.byref(_cache()), C.byref(_query(splits=3))
+    c, q = _cache(), _query(splits=3)
     need = lib.fmi_kv4_attention_ws_bytes(c, q)
     assert need >= 3 * 5 * 4 * 64 * 4
     assert lib.fmi_op_kv4_attention(c, q, A, 256, A, need - 1, None) == -1
@@ -115,23 +136,23 @@ def test_attention_refuses_a_missing_or_small_workspace_and_bad_outputs():
     assert lib.fmi_op_kv4_attention(c, q, A, 256, A + 4, need, None) == -1
     assert lib.fmi_op_kv4_attention(c, q, None, 256, A, need, None) == -1
     assert lib.fmi_op_kv4_attention(c, q, A, 192, A, need, None) == -1
-    assert lib.fmi_kv4_attention_ws_bytes(c, C.byref(_query(splits=1))) == 0
+    assert lib.fmi_kv4_attention_ws_bytes(c, _query(splits=1)) == 0
 
 
 def test_null_arguments_and_empty_calls():
     lib = _lib.load()
-    assert lib.fmi_op_kv4_append(None, C.byref(_rows()), None) == -1
-    assert lib.fmi_op_kv4_append(C.byref(_cache()), None, None) == -1
+    assert lib.fmi_op_kv4_append(None, _rows(), None) == -1
+    assert lib.fmi_op_kv4_append(_cache(), None, None) == -1
     assert lib.fmi_op_kv4_read(None, A, A, 3, A, A, None) == -1
-    assert lib.fmi_op_kv4_read(C.byref(_cache()), None, A, 3, A, A, None) == -1
-    assert lib.fmi_op_kv4_read(C.byref(_cache()), A, A, -3, A, A, None) == -1
-    assert lib.fmi_op_kv4_read(C.byref(_cache()), A, A, 3, A + 2, A, None) == -1
-    assert lib.fmi_op_kv4_attention(None, C.byref(_query()), A, 256, None, 0, None) == -1
+    assert lib.fmi_op_kv4_read(_cache(), None, A, 3, A, A, None) == -1
+    assert lib.fmi_op_kv4_read(_cache(), A, A, -3, A, A, None) == -1
+    assert lib.fmi_op_kv4_read(_cache(), A, A, 3, A + 2, A, None) == -1
+    assert lib.fmi_op_kv4_attention(None, _query(), A, 256, None, 0, None) == -1
     # nothing to do: fine, and nothing is launched
-    assert lib.fmi_op_kv4_append(C.byref(_cache()), C.byref(_rows(rows=0)), None) == 0
-    assert lib.fmi_op_kv4_read(C.byref(_cache()), None, None, 0, None, None, None) == 0
-    assert lib.fmi_op_kv4_attention(C.byref(_cache()), C.byref(_query(total_q=0)), A, 256, None, 0, None) == 0
-    assert lib.fmi_op_kv4_attention(C.byref(_cache()), C.byref(_query(n_seqs=0, q_start_dev=None, kv_len_dev=None)), A, 256,
+    assert lib.fmi_op_kv4_append(_cache(), _rows(rows=0), None) == 0
+    assert lib.fmi_op_kv4_read(_cache(), None, None, 0, None, None, None) == 0
+    assert lib.fmi_op_kv4_attention(_cache(), _query(total_q=0), A, 256, None, 0, None) == 0
+    assert lib.fmi_op_kv4_attention(_cache(), _query(n_seqs=0, q_start_dev=None, kv_len_dev=None), A, 256,
                                     None, 0, None) == 0
 
 
@@ -155,9 +176,7 @@ def test_cache_needs_a_gpu():
 def cache():
     """A cache object whose tensors live on the CPU: good enough for checks that end before any launch."""
     c = kv4.KV4Cache.__new__(kv4.KV4Cache)
-    c.lib, c.device = _lib.load(), torch.device("cpu")
-    c.n_pages, c.n_kv_head, c.head_dim = 4, 2, 64
-    c.pool = torch.zeros(4, 2, 2, 64 * 34, dtype=torch.uint8)
+    c._setup(torch.zeros(4, 2, 2, 64 * 34, dtype=torch.uint8), 64)
     return c
 
 
