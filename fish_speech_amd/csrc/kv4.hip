@@ -65,43 +65,73 @@ __device__ inline float kv4_rstd(double m) {
   return (float)y;
 }
 
-// D / 8 lanes own one (row, head), 8 dims each; a wave takes 64 / (D / 8) consecutive rows of ONE head, so its code
-// bytes are consecutive in the page.  Every rounding is fixed by the definition (sum of squares in fp64, reciprocal
-// norm and both products rounded to fp32, value to bf16; rotation in fp32 without fused products, then bf16), so the
-// stored codes do not depend on how the lanes are arranged.
-template <int D>
+// D / 8 lanes own one (row, head), 8 dims each; a wave takes 64 / (D / 8) consecutive rows of one head, so its code bytes are
+// consecutive in the page, and up to HC heads of one kind (q, k or v) one after the other: indices, page and rotation are
+// looked up once for them, the next head's values are in flight.  grid (chunks of heads; groups of rows).  Every rounding
+// is fixed by the definition (sum of squares in fp64, reciprocal norm and both products rounded to fp32, value to bf16;
+// products of the rotation are exact in fp32, one rounding of their sum, then bf16), so the stored codes do not depend on
+// how the lanes are arranged or on fused products.
+template <int D, bool HALF, int HC>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
-  constexpr int LPH = D / 8, RPW = 64 / LPH;
+  constexpr int LPH = D / 8, RPW = 64 / LPH, BLK = kv4_block_bytes(D);
   const int lane = threadIdx.x & 63, sub = lane % LPH;
-  const int heads = a.H + 2 * a.c.KVH;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int head = (int)(w % heads);
-  const int64_t row64 = (w / heads) * RPW + lane / LPH;
-  const bool in_rows = row64 < a.rows;
-  const int row = in_rows ? (int)row64 : 0;
+  const int qc = (a.H + HC - 1) / HC, kc = (a.c.KVH + HC - 1) / HC, chunk = blockIdx.x;
+  const int kind = chunk < qc ? 0 : chunk < qc + kc ? 1 : 2;   // q, k, v
+  const int h0 = (kind == 0 ? chunk : kind == 1 ? chunk - qc : chunk - qc - kc) * HC;
+  const int h1 = min(h0 + HC, kind == 0 ? a.H : a.c.KVH);
+  const int64_t row64 = (((int64_t)blockIdx.z * 65535 + blockIdx.y) * 4 + (threadIdx.x >> 6)) * RPW + lane / LPH;
+  const bool in_rows = row64 < a.rows;             // rows past the last one read row 0 and are dropped by their position
+  const int64_t row = in_rows ? row64 : 0;
+  const int64_t stride = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
+  const bf16_t* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + row * stride;
+  const bf16_t* nw = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+  const bool rotated = kind != 2 && a.rope && sub * 8 < a.rot;
+  // half layout: the other element of each pair lies rot / 2 dims away, in another lane's chunk
+  const int hr = a.rot / 2;
+  const bool first = sub * 8 < hr;
+  const int psub = HALF && rotated ? (first ? sub + hr / 8 : sub - hr / 8) : sub;
+  u32x4 nx = *reinterpret_cast<const u32x4*>(src + h0 * D + sub * 8), nxp;
+  if (HALF) nxp = *reinterpret_cast<const u32x4*>(src + h0 * D + psub * 8);
   const int seq = in_rows ? a.row_seq[row] : -1;
   const bool seq_ok = seq >= 0 && seq < a.c.n_slots;
   const int pos = seq_ok ? (a.row_pos ? a.row_pos[row] : a.slot_pos[seq]) : -1;
-  const int64_t limit = (int64_t)a.c.max_pages * KV_PAGE;
-  const bool valid = pos >= 0 && pos < limit && (!a.rope || pos < a.rope_len);
-
-  const int kind = head < a.H ? 0 : head < a.H + a.c.KVH ? 1 : 2;   // q, k, v
-  const int hh = kind == 0 ? head : kind == 1 ? head - a.H : head - a.H - a.c.KVH;
-  const bf16_t* src = kind == 0 ? a.q + row * a.q_stride : kind == 1 ? a.k + row * a.k_stride : a.v + row * a.v_stride;
-  src += (int64_t)hh * D;
-  u32x4 x = *reinterpret_cast<const u32x4*>(src + sub * 8);
-
-  if (kind != 2) {
-    const bf16_t* nw = kind == 0 ? a.q_norm : a.k_norm;
-    const bool rot = a.rope && sub * 8 < a.rot && valid;
-    // half layout: the other element of each pair lies rot / 2 dims away, in another lane's chunk
-    const int hr = a.rot / 2;
-    const bool first = sub * 8 < hr;
-    const int psub = rot && a.half ? (first ? sub + hr / 8 : sub - hr / 8) : sub;
-    u32x4 xp = x;
-    if (rot && a.half) xp = *reinterpret_cast<const u32x4*>(src + psub * 8);
+  const bool valid = pos >= 0 && pos < (a.rope ? min(a.c.max_pages * KV_PAGE, a.rope_len) : a.c.max_pages * KV_PAGE);
+  const bool rot = rotated && valid;
+  int page = kind != 0 && valid ? a.c.block_table[(int64_t)seq * a.c.max_pages + pos / KV_PAGE] : -1;
+  if (kind != 0 && valid && a.slot_done && a.slot_done[seq]) page = -1;
+  float wv[8], wp[8], cs[8], sn[8];
+  if (nw) {
+    const u32x4 w0 = *reinterpret_cast<const u32x4*>(nw + sub * 8), w1 = *reinterpret_cast<const u32x4*>(nw + psub * 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      wv[i] = i & 1 ? bf_hi(w0[i >> 1]) : bf_lo(w0[i >> 1]);
+      if (HALF) wp[i] = i & 1 ? bf_hi(w1[i >> 1]) : bf_lo(w1[i >> 1]);
+    }
+  }
+  if (rot) {
+    // interleaved: cs / sn [i] of pair i (i < 4); half: of this lane's element i, the sine negated for the first of a pair
+    const bf16_t* tab = a.rope + (int64_t)pos * a.rot + (HALF ? (first ? sub * 8 : sub * 8 - hr) * 2 : sub * 8);
+    uint32_t t[8];
+    *reinterpret_cast<u32x4*>(t) = *reinterpret_cast<const u32x4*>(tab);
+    if (HALF) *reinterpret_cast<u32x4*>(t + 4) = *reinterpret_cast<const u32x4*>(tab + 8);
+#pragma unroll
+    for (int i = 0; i < (HALF ? 8 : 4); ++i) {
+      cs[i] = bf_lo(t[i]);
+      sn[i] = HALF && first ? -bf_hi(t[i]) : bf_hi(t[i]);
+    }
+  }
+  const bool store = page >= 0 && page < a.c.n_pages;
+  const int tok = pos % KV_PAGE;
+  // (a lane without a page never uses its addresses)
+  uint8_t* blk = a.c.pool + ((store ? (int64_t)page : 0) * a.c.KVH * 2 + (kind - 1)) * BLK;
+#pragma unroll 1
+  for (int h = h0; h < h1; ++h) {
+    u32x4 x = nx, xp = nxp;
+    if (HC > 1 && h + 1 < h1) {
+      nx = *reinterpret_cast<const u32x4*>(src + (h + 1) * D + sub * 8);
+      if (HALF) nxp = *reinterpret_cast<const u32x4*>(src + (h + 1) * D + psub * 8);
+    }
     if (nw) {
-      const u32x4 wv = *reinterpret_cast<const u32x4*>(nw + sub * 8), wp = *reinterpret_cast<const u32x4*>(nw + psub * 8);
       double ss = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -113,69 +143,45 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
       ss += xor_lane_d<2>(ss, lane);
       if (LPH > 4) ss += xor_lane_d<4>(ss, lane);
       if (LPH > 8) ss += xor_lane_d<8>(ss, lane);
-      const float rstd = kv4_rstd(ss / (double)D + a.eps);
+      const float rstd = kv4_rstd(ss * (1.0 / D) + a.eps);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        x[i] = kv4_pk_bf16(__fmul_rn(__fmul_rn(bf_lo(x[i]), rstd), bf_lo(wv[i])),
-                           __fmul_rn(__fmul_rn(bf_hi(x[i]), rstd), bf_hi(wv[i])));
-        xp[i] = kv4_pk_bf16(__fmul_rn(__fmul_rn(bf_lo(xp[i]), rstd), bf_lo(wp[i])),
-                            __fmul_rn(__fmul_rn(bf_hi(xp[i]), rstd), bf_hi(wp[i])));
+        x[i] = kv4_pk_bf16(bf_lo(x[i]) * rstd * wv[2 * i], bf_hi(x[i]) * rstd * wv[2 * i + 1]);
+        if (HALF) xp[i] = kv4_pk_bf16(bf_lo(xp[i]) * rstd * wp[2 * i], bf_hi(xp[i]) * rstd * wp[2 * i + 1]);
       }
     }
     if (rot) {
-      const bf16_t* tab = a.rope + (int64_t)pos * a.rot;
-      if (!a.half) {
-        const u32x4 cs = *reinterpret_cast<const u32x4*>(tab + sub * 8);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x0 = bf_lo(x[i]), x1 = bf_hi(x[i]), c = bf_lo(cs[i]), s = bf_hi(cs[i]);
-          x[i] = kv4_pk_bf16(__fsub_rn(__fmul_rn(x0, c), __fmul_rn(x1, s)), __fadd_rn(__fmul_rn(x1, c), __fmul_rn(x0, s)));
-        }
-      } else {
-        const bf16_t* tp = tab + (first ? sub * 8 : sub * 8 - hr) * 2;
-        const u32x4 c0 = *reinterpret_cast<const u32x4*>(tp), c1 = *reinterpret_cast<const u32x4*>(tp + 8);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint32_t csa = i < 2 ? c0[2 * i] : c1[2 * i - 4], csb = i < 2 ? c0[2 * i + 1] : c1[2 * i - 3];
-          float r[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const float me = j ? bf_hi(x[i]) : bf_lo(x[i]), other = j ? bf_hi(xp[i]) : bf_lo(xp[i]);
-            const float c = bf_lo(j ? csb : csa), s = bf_hi(j ? csb : csa);
-            r[j] = first ? __fsub_rn(__fmul_rn(me, c), __fmul_rn(other, s)) : __fadd_rn(__fmul_rn(me, c), __fmul_rn(other, s));
-          }
-          x[i] = kv4_pk_bf16(r[0], r[1]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const float x0 = bf_lo(x[i]), x1 = bf_hi(x[i]);
+        if (!HALF) x[i] = kv4_pk_bf16(x0 * cs[i] - x1 * sn[i], x1 * cs[i] + x0 * sn[i]);
+        else x[i] = kv4_pk_bf16(x0 * cs[2 * i] + bf_lo(xp[i]) * sn[2 * i], x1 * cs[2 * i + 1] + bf_hi(xp[i]) * sn[2 * i + 1]);
       }
     }
-  }
-  if (kind == 0) {
-    if (valid) *reinterpret_cast<u32x4*>(a.q_out + row * a.q_out_stride + (int64_t)hh * D + sub * 8) = x;
-    return;
-  }
-  // ---- quantise: 4 lanes hold a 32-dim block
-  uint32_t top = 0;
+    if (kind == 0) {
+      if (valid) *reinterpret_cast<u32x4*>(a.q_out + row * a.q_out_stride + h * D + sub * 8) = x;
+      continue;
+    }
+    // ---- quantise: 4 lanes hold a 32-dim block
+    uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) top = max(top, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
-  top = max(top, (uint32_t)xor_lane<1>((int)top, lane));
-  top = max(top, (uint32_t)xor_lane<2>((int)top, lane));
-  const bool finite = top < 0x7f80u;
-  // max = 1.f * 2^(exp - 127): the power with max <= 7 * 2^e is exp - 127 - 2, one more above f = 1.75
-  const int b = min(max((int)(top >> 7) - 2 + ((top & 0x7fu) > 0x60u ? 1 : 0), KV4_MIN_SCALE), KV4_MAX_SCALE);
-  const float sc = kv4_scale((uint32_t)b);
-  uint32_t codes = 0;
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[0]), sc, 0);
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[1]), sc, 1);
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[2]), sc, 2);
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[3]), sc, 3);
-  if (!valid || (a.slot_done && a.slot_done[seq])) return;
-  const int page = a.c.block_table[(int64_t)seq * a.c.max_pages + pos / KV_PAGE];
-  if (page < 0 || page >= a.c.n_pages) return;
-  constexpr int BLK = kv4_block_bytes(D);
-  const int tok = pos % KV_PAGE;
-  uint8_t* blk = a.c.pool + (((int64_t)page * a.c.KVH + hh) * 2 + (kind - 1)) * BLK;
-  *reinterpret_cast<uint32_t*>(blk + tok * (D / 2) + sub * 4) = finite ? codes : 0u;
-  if ((sub & 3) == 0) blk[KV_PAGE * (D / 2) + tok * (D / 32) + sub / 4] = (uint8_t)(finite ? b : KV4_NAN_SCALE);
+    for (int i = 0; i < 4; ++i) top = max(top, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
+    top = max(top, (uint32_t)xor_lane<1>((int)top, lane));
+    top = max(top, (uint32_t)xor_lane<2>((int)top, lane));
+    const bool finite = top < 0x7f80u;
+    // max = 1.f * 2^(exp - 127): the power with max <= 7 * 2^e is exp - 127 - 2, one more above f = 1.75
+    const int b = min(max((int)(top >> 7) - 2 + ((top & 0x7fu) > 0x60u ? 1 : 0), KV4_MIN_SCALE), KV4_MAX_SCALE);
+    const float sc = kv4_scale((uint32_t)b);
+    uint32_t codes = 0;
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[0]), sc, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[1]), sc, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[2]), sc, 2);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[3]), sc, 3);
+    if (!store) continue;
+    uint8_t* hb = blk + (int64_t)h * 2 * BLK;
+    *reinterpret_cast<uint32_t*>(hb + tok * (D / 2) + sub * 4) = finite ? codes : 0u;
+    if ((sub & 3) == 0) hb[KV_PAGE * (D / 2) + tok * (D / 32) + sub / 4] = (uint8_t)(finite ? b : KV4_NAN_SCALE);
+  }
 }
 
 static int kv4_check_cache(const Kv4Cache& c) {
@@ -183,7 +189,7 @@ static int kv4_check_cache(const Kv4Cache& c) {
   FMI_REQUIRE(c.D == 32 || c.D == 64 || c.D == 128, "kv4: head_dim %d unsupported (32/64/128)", c.D);
   FMI_REQUIRE(c.KVH >= 1 && c.n_pages >= 1 && c.n_slots >= 1 && c.max_pages >= 1,
               "kv4: n_kv_head %d, n_pages %d, n_seqs %d and max_pages %d must be positive", c.KVH, c.n_pages, c.n_slots, c.max_pages);
-  FMI_REQUIRE(c.max_pages <= (1 << 24), "kv4: max_pages %d exceeds 2^24", c.max_pages);
+  FMI_REQUIRE(c.max_pages <= (1 << 24) && c.KVH <= (1 << 16), "kv4: max_pages %d, n_kv_head %d: at most 2^24, 2^16", c.max_pages, c.KVH);
   FMI_REQUIRE(((uintptr_t)c.pool & 15) == 0 && ((uintptr_t)c.block_table & 3) == 0, "kv4: misaligned pool or block table");
   return FMI_OK;
 }
@@ -195,6 +201,12 @@ static int kv4_check_rows(const char* what, const void* p, int64_t stride, int h
   return FMI_OK;
 }
 
+// grid of the row kernels: (heads, groups of `per` rows); y holds 65535 groups, z the rest
+static dim3 kv4_row_grid(int64_t heads, int rows, int per) {
+  const int64_t groups = ((int64_t)rows + per - 1) / per;
+  return dim3((unsigned)heads, (unsigned)std::min<int64_t>(groups, 65535), (unsigned)((groups + 65534) / 65535));
+}
+
 int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
   FMI_CHECK(kv4_check_cache(a.c));
   const int D = a.c.D;
@@ -204,7 +216,7 @@ int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
   FMI_CHECK(kv4_check_rows("v", a.v, a.v_stride, a.c.KVH, D));
   FMI_REQUIRE(a.row_seq && (a.row_pos || a.slot_pos), "kv4 append: null row indices");
   if (a.q) {
-    FMI_REQUIRE(a.H >= 1, "kv4 append: q without query heads");
+    FMI_REQUIRE(a.H >= 1 && a.H <= (1 << 16), "kv4 append: q of %d query heads (1 to 2^16)", a.H);
     FMI_CHECK(kv4_check_rows("q", a.q, a.q_stride, a.H, D));
     FMI_CHECK(kv4_check_rows("q_out", a.q_out, a.q_out_stride, a.H, D));
   } else {
@@ -215,13 +227,20 @@ int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
     FMI_REQUIRE(((uintptr_t)a.rope & 15) == 0 && a.rope_len >= 1, "kv4 append: empty or misaligned rotation table");
     FMI_REQUIRE(a.rot >= 16 && a.rot <= D && a.rot % 16 == 0, "kv4 append: %d rotated dims (a multiple of 16 up to head_dim %d)", a.rot, D);
   }
-  const int rpw = 64 / (D / 8);
-  const int64_t waves = ((int64_t)a.rows + rpw - 1) / rpw * (a.H + 2 * a.c.KVH);
-  const int64_t blocks = (waves + 3) / 4;
-  FMI_REQUIRE(blocks < (int64_t)1 << 31, "kv4 append: too many rows");
-  if (D == 128) hipLaunchKernelGGL((kv4_append_kernel<128>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-  else if (D == 64) hipLaunchKernelGGL((kv4_append_kernel<64>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((kv4_append_kernel<32>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+  const bool half = a.rope && a.half, many = (int64_t)a.rows * (a.H + 2 * a.c.KVH) * D > (int64_t)1 << 23;
+  const int hc = many ? 8 : 1;
+  const dim3 grid = kv4_row_grid((a.H + hc - 1) / hc + 2 * ((a.c.KVH + hc - 1) / hc), a.rows, 4 * (64 / (D / 8)));
+#define FMI_KV4_APPEND(D_)                                                                                             \
+  do {                                                                                                                 \
+    if (many && half) hipLaunchKernelGGL((kv4_append_kernel<D_, true, 8>), grid, dim3(256), 0, s, a);                  \
+    else if (many) hipLaunchKernelGGL((kv4_append_kernel<D_, false, 8>), grid, dim3(256), 0, s, a);                    \
+    else if (half) hipLaunchKernelGGL((kv4_append_kernel<D_, true, 1>), grid, dim3(256), 0, s, a);                     \
+    else hipLaunchKernelGGL((kv4_append_kernel<D_, false, 1>), grid, dim3(256), 0, s, a);                              \
+  } while (0)
+  if (D == 128) FMI_KV4_APPEND(128);
+  else if (D == 64) FMI_KV4_APPEND(64);
+  else FMI_KV4_APPEND(32);
+#undef FMI_KV4_APPEND
   FMI_CHECK_HIP(hipGetLastError());
   return FMI_OK;
 }
@@ -235,10 +254,8 @@ template <int D>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadArgs a) {
   constexpr int LPH = D / 8, RPW = 64 / LPH, BLK = kv4_block_bytes(D);
   const int lane = threadIdx.x & 63, sub = lane % LPH;
-  const int heads = 2 * a.c.KVH;
-  const int64_t w = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int head = (int)(w % heads), isv = head & 1, kh = head >> 1;
-  const int64_t row = (w / heads) * RPW + lane / LPH;
+  const int isv = blockIdx.x & 1, kh = blockIdx.x >> 1;
+  const int64_t row = (((int64_t)blockIdx.z * 65535 + blockIdx.y) * 4 + (threadIdx.x >> 6)) * RPW + lane / LPH;
   if (row >= a.rows) return;
   const int seq = a.row_seq ? a.row_seq[row] : a.seq0, pos = a.row_seq ? a.row_pos[row] : (int)row;
   u32x4 x = {0, 0, 0, 0};
@@ -262,12 +279,10 @@ int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s) {
   FMI_REQUIRE(!a.row_seq == !a.row_pos, "kv4 read: null row indices");
   FMI_CHECK(kv4_check_rows("k", a.k, (int64_t)a.c.KVH * D, a.c.KVH, D));
   FMI_CHECK(kv4_check_rows("v", a.v, (int64_t)a.c.KVH * D, a.c.KVH, D));
-  const int rpw = 64 / (D / 8);
-  const int64_t blocks = (((int64_t)a.rows + rpw - 1) / rpw * (2 * a.c.KVH) + 3) / 4;
-  FMI_REQUIRE(blocks < (int64_t)1 << 31, "kv4 read: too many rows");
-  if (D == 128) hipLaunchKernelGGL((kv4_read_kernel<128>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-  else if (D == 64) hipLaunchKernelGGL((kv4_read_kernel<64>), dim3((unsigned)blocks), dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((kv4_read_kernel<32>), dim3((unsigned)blocks), dim3(256), 0, s, a);
+  const dim3 grid = kv4_row_grid(2 * (int64_t)a.c.KVH, a.rows, 4 * (64 / (D / 8)));
+  if (D == 128) hipLaunchKernelGGL((kv4_read_kernel<128>), grid, dim3(256), 0, s, a);
+  else if (D == 64) hipLaunchKernelGGL((kv4_read_kernel<64>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((kv4_read_kernel<32>), grid, dim3(256), 0, s, a);
   FMI_CHECK_HIP(hipGetLastError());
   return FMI_OK;
 }
@@ -600,7 +615,9 @@ __device__ inline uint32_t kv4_pk_f16(float lo, float hi) {
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a) {
   constexpr int NT = 64 * NW, BLK = kv4_block_bytes(D), NB = D / 32, TC = 32 * NW;
-  constexpr int KROW = D * 2 + 16, VROW = D * 2 + 32;      // padded LDS rows: neighbouring keys in different banks
+  // LDS rows: K reads take 16 keys at 16 bytes each (rows 4 banks apart), V reads 4 keys at 2 x 32 bytes (16 banks apart).
+  // V's writes then meet in a bank unless the four 16-byte words of a piece go out in an order that differs by key.
+  constexpr int KROW = D * 2 + 16, VROW = D * 2 + (D > 32 ? 64 : 0);
   constexpr int PIECES = 2 * KV_PAGE * NB;                  // 16-byte pieces (32 codes) of K and V of a page
   constexpr int PPT = (PIECES + NT - 1) / NT;
   __shared__ __attribute__((aligned(16))) unsigned char s_k[2][KV_PAGE * KROW];
@@ -609,10 +626,13 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int KVH = a.c.KVH, G = a.H / KVH;
+  // heads fastest (the work-groups of a kv head's keys share an XCD and its L2 when there are 8), then a sequence's tiles from
+  // the one with the most keys down, then sequences (sequences before tiles: 326 us for 240 on two ragged 2k-token prompts
+  // over 4k keys, 129 for 96 on four ragged prompts of up to 2k; even at best elsewhere)
   const int kvh = blockIdx.x % KVH, z = blockIdx.y;
   const Kv4Span sp = kv4_span(a, blockIdx.z);
   const int cols = sp.nq * G, tiles = (cols + TC - 1) / TC;
-  const int tile = tiles - 1 - (int)(blockIdx.x / KVH);    // the tiles with the most keys first
+  const int tile = tiles - 1 - (int)(blockIdx.x / KVH);
   if (tile < 0) return;
   const int col0 = tile * TC, pos0 = sp.kv - sp.nq;
   const int np = kv4_tile_pages(sp, G, col0, TC), nz = kv4_attn_ranges(a, np);
@@ -632,7 +652,11 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   {
     const bf16_t* qp = a.q + qrow * a.q_stride + (int64_t)head * D + h * 8;
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(qp + kk * 16);
+    for (int kk = 0; kk < D / 16; ++kk) {
+      u32x4 t = *reinterpret_cast<const u32x4*>(qp + kk * 16);
+      if (a.scale < 0.f) t ^= 0x80008000u;      // the largest product is then the largest score for either sign of the scale
+      qf[kk] = *reinterpret_cast<bf16x8*>(&t);
+    }
   }
   f32x16 o[NB];
 #pragma unroll
@@ -641,7 +665,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   float m = -FLT_MAX, l = 0.f;
   int E = KV4_MIN_SCALE;
-  const float sl = a.scale * 1.4426950408889634f;
+  const float sl = fabsf(a.scale) * 1.4426950408889634f;   // scores in units of log2
 
   u32x4 code[PPT];
   uint32_t scale[PPT], vtok = 0;                            // vtok: the V scales of token `lane`
@@ -695,10 +719,13 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
             if (bad) atomicMin(&s_nan[part], pg * KV_PAGE + key);
             // (2^-31 and below round every value to 0; a masked block must not pass its scale on: 255 gives NaN even for 0)
             const float vs = kv4_scale(use && !bad ? (uint32_t)max((int)scale[i] - E + 127, 96) : 127u);
+            u32x4 cw = use && !bad ? code[i] : (u32x4){0, 0, 0, 0};
+            const int turn = NB == 4 ? key & 3 : NB == 2 ? (key & 1) | ((key >> 1) & 2) : (key >> 2) & 3;
+            if (turn & 1) cw = (u32x4){cw[1], cw[2], cw[3], cw[0]};
+            if (turn & 2) cw = (u32x4){cw[2], cw[3], cw[0], cw[1]};
+            unsigned char* vw = &s_v[it][key * VROW + part * 64];
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-              *reinterpret_cast<u32x4*>(&s_v[it][key * VROW + part * 64 + w * 16]) =
-                  kv4_unpack8_f16(use && !bad ? code[i][w] : 0u, vs);
+            for (int w = 0; w < 4; ++w) *reinterpret_cast<u32x4*>(vw + ((w + turn) & 3) * 16) = kv4_unpack8_f16(cw[w], vs);
           }
         }
       }
@@ -706,52 +733,74 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
     __syncthreads();      // the page is staged; and every wave is done with the page before the previous one (same buffer)
     if (pg + 1 < p_hi) fetch(pg + 1, next_page);
     if (there && pg * KV_PAGE < any_see) {
+      // V^T fragments of 16 keys: lanes 4 r .. 4 r + 3 of a 16-lane group name row (key) r; lane i of the group gets dim i of
+      // the 4 rows.  The first are requested before the scores, the others a product ahead.
+      const unsigned char* vr = &s_v[it][(4 * h + ((lane & 15) >> 2)) * VROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8];
+      auto read_v = [&](int st, f16x8_t* f) {
+#pragma unroll
+        for (int dt = 0; dt < NB; ++dt) {
+          const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + st * 16 * VROW + dt * 64));
+          const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + (st * 16 + 8) * VROW + dt * 64));
+          const bf16x8 t = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+          f[dt] = __builtin_bit_cast(f16x8_t, t);
+        }
+      };
+      f16x8_t vf[NB];
       // ---- scores
       f32x16 sacc[2];
+      bf16x8 kf[2][D / 16];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sacc[kt][i] = 0.f;
-        const unsigned char* kr = &s_k[it][(kt * 32 + c) * KROW + h * 16];
+      for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(*reinterpret_cast<const bf16x8*>(kr + kk * 32), qf[kk], sacc[kt], 0, 0, 0);
-      }
+          kf[kt][kk] = *reinterpret_cast<const bf16x8*>(&s_k[it][(kt * 32 + c) * KROW + h * 16 + kk * 32]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sacc[0][i] = sacc[1][i] = 0.f;
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt) sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kt][kk], qf[kk], sacc[kt], 0, 0, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 2 * (D / 16), 0);   // the reads first
+      __builtin_amdgcn_sched_group_barrier(0x008, 2 * (D / 16), 0);
       // ---- softmax: register i of tile kt is key kt * 32 + 8 (i / 4) + 4 h + i % 4 of column c
-      float mx = -FLT_MAX;
-      if (pg * KV_PAGE + KV_PAGE > all_see) {
-        const int lim = vis - pg * KV_PAGE - 4 * h;
+      const bool part = pg * KV_PAGE + KV_PAGE > all_see;
+      const int lim = vis - pg * KV_PAGE - 4 * h;
+      float mx = -INFINITY;
+      if (part) {       // an unseen key's score is minus infinity whatever its K holds
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const bool see = kt * 32 + 8 * (i >> 2) + (i & 3) < lim;
-            // the scaled score of an unseen key is minus infinity whatever its K holds
-            sacc[kt][i] = see ? sacc[kt][i] * sl : -INFINITY;
-            mx = fmaxf(mx, sacc[kt][i]);
-          }
-      } else {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            sacc[kt][i] *= sl;
-            mx = fmaxf(mx, sacc[kt][i]);
-          }
+          for (int i = 0; i < 16; ++i)
+            if (!(kt * 32 + 8 * (i >> 2) + (i & 3) < lim)) sacc[kt][i] = -INFINITY;
       }
-      mx = max_swap32(mx);
-      const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sacc[kt][i]);
+      mx = max_swap32(mx) * sl;
+      // the reference m moves only when a score exceeds it by 2^8: weights up to 256 are as exact in fp16 as weights up to 1,
+      // and O is seldom rescaled.  (mx is NaN for minus infinity times a scale of 0: no key seen, m stays.)
+      const float mn = mx > m + 8.f ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn);
       float ps = 0.f;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          sacc[kt][i] = __builtin_amdgcn_exp2f(sacc[kt][i] - mn);
-          ps += sacc[kt][i];
-        }
+        for (int i = 0; i < 16; ++i) sacc[kt][i] = __builtin_amdgcn_exp2f(fmaf(sacc[kt][i], sl, -mn));
+      if (part && sl == 0.f) {      // (0 times minus infinity)
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (!(kt * 32 + 8 * (i >> 2) + (i & 3) < lim)) sacc[kt][i] = 0.f;
+      }
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) ps += sacc[kt][i];
       l = l * corr + ps;
       m = mn;
       const float oc = corr * grow;
+      read_v(0, vf);
       if (__builtin_amdgcn_ballot_w64(oc != 1.f)) {
 #pragma unroll
         for (int dt = 0; dt < NB; ++dt)
@@ -764,17 +813,16 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
       for (int st = 0; st < 4; ++st)
 #pragma unroll
         for (int i = 0; i < 4; ++i) pf[st][i] = kv4_pk_f16(sacc[st >> 1][(st & 1) * 8 + 2 * i], sacc[st >> 1][(st & 1) * 8 + 2 * i + 1]);
-      // lanes 4 r .. 4 r + 3 of a 16-lane group name row (key) r; lane i of the group gets dim i of the 4 rows
-      const unsigned char* vr = &s_v[it][(4 * h + ((lane & 15) >> 2)) * VROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8];
 #pragma unroll
-      for (int st = 0; st < 4; ++st)
+      for (int st = 0; st < 4; ++st) {
+        f16x8_t vn[NB];
+        if (st < 3) read_v(st + 1, vn);
 #pragma unroll
-        for (int dt = 0; dt < NB; ++dt) {
-          const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + st * 16 * VROW + dt * 64));
-          const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + (st * 16 + 8) * VROW + dt * 64));
-          const bf16x8 vf = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf), __builtin_bit_cast(f16x8_t, pf[st]), o[dt], 0, 0, 0);
-        }
+        for (int dt = 0; dt < NB; ++dt)
+          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[dt], __builtin_bit_cast(f16x8_t, pf[st]), o[dt], 0, 0, 0);
+#pragma unroll
+        for (int dt = 0; dt < NB; ++dt) vf[dt] = vn[dt];
+      }
     } else if (grow != 1.f) {
 #pragma unroll
       for (int dt = 0; dt < NB; ++dt)
@@ -921,7 +969,7 @@ int launch_kv4_attn(const Kv4AttnArgs& a_, hipStream_t s) {
   Kv4AttnArgs a = a_;
   FMI_CHECK(kv4_check_cache(a.c));
   const int D = a.c.D;
-  FMI_REQUIRE(a.H >= 1 && a.H % a.c.KVH == 0, "kv4 attention: %d query heads over %d kv heads", a.H, a.c.KVH);
+  FMI_REQUIRE(a.H >= 1 && a.H <= (1 << 16) && a.H % a.c.KVH == 0, "kv4 attention: %d query heads over %d kv heads", a.H, a.c.KVH);
   FMI_REQUIRE(a.n_seqs >= 0 && a.n_seqs <= 65535 && a.total_q >= 0 && a.max_q >= 0 && a.max_kv >= 0,
               "kv4 attention: bad sizes (n_seqs %d, total_q %d, max_q %d, max_kv %d)", a.n_seqs, a.total_q, a.max_q, a.max_kv);
   if (a.n_seqs == 0 || a.total_q == 0 || a.max_q == 0) return FMI_OK;

@@ -186,7 +186,6 @@ class KV4Cache:
         the sequences, the block table or the pool read as 0."""
         rows = row_seq.shape[0] if row_seq.dim() == 1 else -1
         sp, pp = self._index("row_seq", row_seq, rows), self._index("row_pos", row_pos, rows)
-        k = torch.empty(rows, self.n_kv_head, self.head_dim, dtype=_BF16, device=self.device)
-        v = torch.empty(rows, self.n_kv_head, self.head_dim, dtype=_BF16, device=self.device)
+        k, v = torch.empty(2, rows, self.n_kv_head, self.head_dim, dtype=_BF16, device=self.device).unbind(0)
         self._call(self.lib.fmi_op_kv4_read, self._cache(block_table), sp, pp, rows, k.data_ptr(), v.data_ptr())
         return k, v
