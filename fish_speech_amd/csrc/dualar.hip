@@ -388,7 +388,8 @@ int attn_kv4(fmi_dualar* h, const LayerW& w, int layer, int rows, const int32_t*
     a.q_start = h->kv4_seq; a.kv_len = h->kv4_seq + h->max_batch + 1; a.seq_slot = h->kv4_seq + 2 * h->max_batch + 1;
     a.n_seqs = h->kv4_n; a.max_q = h->kv4_max_q; a.splits = 1; a.form = 2;
   } else {
-    a.seq_slot = row_slot; a.n_seqs = rows; a.max_q = 1; a.splits = KV4_SPLITS; a.form = 1; a.part = h->kv4_part;
+    a.seq_slot = row_slot; a.n_seqs = rows; a.max_q = 1; a.form = 1; a.part = h->kv4_part;
+    a.splits = (h->attn_mask & 2) ? KV4_SPLITS : 1;   // (bit 2 unset: no row is long enough to be split, the merge launch is saved)
   }
   FMI_CHECK(launch_kv4_attn(a, s));
   h->launches += a.splits > 1 ? 3 : 2;
@@ -469,6 +470,14 @@ int block_fast(fmi_dualar* h, const LayerW& w, int layer, bf16_t* x, int B, int 
   FMI_CHECK(linear(h, x, d.dim, w.w13, w.ffn_norm, nullptr, 0, ws.act, d.ffn, B, 2 * d.ffn, d.dim, EPI_SILU, s, w.q_w13, w.s_w13));
   FMI_CHECK(linear(h, ws.act, d.ffn, w.w2, nullptr, x, d.dim, x, d.dim, B, d.dim, d.ffn, EPI_RESIDUAL, s, w.q_w2, w.s_w2, w.r_w2));
   return FMI_OK;
+}
+
+// attn_mask of a frame or frames in which a row's position reaches `last`, the lowest being `first`: which decode attention
+// kernels the frames launch (bf16 cache) or whether rows are split over key ranges (4-bit cache)
+int attn_mask_of(const fmi_dualar* h, int first, int last) {
+  if (h->kv_bits == 4) return last + 1 > (KV4_SINGLE_PAGES - 1) * KV_PAGE ? 2 : 1;
+  if (h->attn_long_thr <= 0) return 1;
+  return (first < h->attn_long_thr ? 1 : 0) | (last >= h->attn_long_thr ? 2 : 0);
 }
 
 // everything after the slow transformer for B utterances whose last hidden rows are xl[B][dim]:
@@ -1215,15 +1224,8 @@ int fmi_dualar_decode(fmi_dualar* h, int n, const int32_t* slot_ids, int n_frame
   // which decode-attention kernels the frames of this call need: the VALU kernel if some slot is below the threshold
   // when the call starts, the MFMA pair if some slot reaches it before the call ends (each row then picks by its own
   // position; a launch whose rows are all in the other regime returns at once)
-  int mask = 1;
-  if (h->attn_long_thr > 0) {
-    mask = 0;
-    for (int i = 0; i < n; ++i) {
-      const int p = h->pos_host[slot_ids[i]];
-      if (p < h->attn_long_thr) mask |= 1;
-      if (p + n_frames > h->attn_long_thr) mask |= 2;
-    }
-  }
+  int mask = 0;
+  for (int i = 0; i < n; ++i) mask |= attn_mask_of(h, h->pos_host[slot_ids[i]], h->pos_host[slot_ids[i]] + n_frames - 1);
   h->attn_mask = mask;
   hipGraphExec_t exec = nullptr;
   if (h->use_graph && !h->trace) {
@@ -1352,7 +1354,7 @@ int fmi_dualar_step(fmi_dualar* h, int slot, const int32_t* x_dev, int S, int po
     if (prev_dev)
       FMI_CHECK_HIP(hipMemcpyAsync(h->st.window + (int64_t)slot * ncb1 * RAS_WIN, prev_dev,
                                    (size_t)ncb1 * RAS_WIN * 4, hipMemcpyDeviceToDevice, s));
-    h->attn_mask = (h->attn_long_thr > 0 && pos0 >= h->attn_long_thr) ? 2 : 1;
+    h->attn_mask = attn_mask_of(h, pos0, pos0);
     FMI_CHECK(decode_frame(h, 1, s));
   }
   FMI_CHECK_HIP(hipMemcpyAsync(out_dev, h->st.cur + (int64_t)slot * ncb1, ncb1 * 4, hipMemcpyDeviceToDevice, s));
@@ -1383,7 +1385,7 @@ int fmi_dualar_forward_slow(fmi_dualar* h, int slot, const int32_t* x_dev, int S
     h->row_slot_host.clear();
     FMI_CHECK_HIP(hipMemcpyAsync(h->ws.row_slot, &slot, 4, hipMemcpyHostToDevice, s));
     FMI_CHECK_HIP(hipStreamSynchronize(s));
-    h->attn_mask = (h->attn_long_thr > 0 && pos0 >= h->attn_long_thr) ? 2 : 1;
+    h->attn_mask = attn_mask_of(h, pos0, pos0);
     FMI_CHECK(decode_frame(h, 1, s, true));
   }
   if (logits_out_dev)

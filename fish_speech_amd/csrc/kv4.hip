@@ -315,10 +315,14 @@ __device__ inline int kv4_tile_pages(const Kv4Span& sp, int G, int col0, int til
   const int nk = min(sp.kv - sp.nq + min(col0 + tile_cols - 1, sp.nq * G - 1) / G + 1, sp.cached);
   return nk > 0 ? (nk + KV_PAGE - 1) / KV_PAGE : 0;
 }
-// the ranges a tile of np pages really uses, at least KV4_MIN_PAGES each (one block per wave of a narrow tile): a function of
-// the tile alone.  One range: its work-group writes the output itself and the merge passes the tile's rows by.
+// the ranges a tile of np pages really uses: a function of the tile alone.  One range: its work-group writes the output itself
+// and the merge passes the tile's rows by.  Below KV4_SINGLE_PAGES it is one (8 x 512 keys 7.5 us, in two ranges and a merge
+// 9.1; 8 x 1k 10.5 and 9.9; 8 x 2k 16.3 and 12.7), above it a range has KV4_MIN_PAGES at least (a block per wave of a narrow
+// tile).
 constexpr int KV4_MIN_PAGES = 4;
-__device__ inline int kv4_attn_ranges(const Kv4AttnArgs& a, int np) { return max(1, min(a.splits, np / KV4_MIN_PAGES)); }
+__device__ inline int kv4_attn_ranges(const Kv4AttnArgs& a, int np) {
+  return np < KV4_SINGLE_PAGES ? 1 : max(1, min(a.splits, np / KV4_MIN_PAGES));
+}
 
 // partial states of the key ranges: (m, l) pairs [splits][total_q * H][2], then O [splits][total_q * H][D]
 __device__ inline float* kv4_part_ml(const Kv4AttnArgs& a, int z, int64_t idx) {
@@ -387,28 +391,28 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   const int b_lo = (int)((int64_t)z * np / nz) * 2, b_hi = (int)((int64_t)(z + 1) * np / nz) * 2;
   const int32_t* bt = a.c.block_table + (int64_t)sp.slot * a.c.max_pages;
 
-  // K and V codes and scales of one block; a missing page reads page 0 and is skipped later
+  // K and V codes and scales of one block; a missing page reads page 0 and is skipped later.  A lane's place in the block is
+  // fixed: 32-bit offsets from a scalar base.
   u32x4 vcode[VPASS];
   uint32_t kcode[2][KS], kscale[2], vscale[VPASS];
+  const uint32_t k_off = c * (D / 2) + g * (D / 8), ks_off = c * NB + g * NB / 4;
+  const uint32_t vkey = VP <= KB ? lane / VL : min(lane, KB - 1), v_off = vkey * (D / 2) + lane % VL * 16, vs_off = vkey * NB + lane % VL;
   auto fetch = [&](int kb, int page) {
-    const int pg = page >= 0 && page < a.c.n_pages ? page : 0;
+    const int pg = page >= 0 && page < a.c.n_pages ? page : 0, tok0 = kb & 1 ? KB : 0;
     const uint8_t* kblk = a.c.pool + ((int64_t)pg * KVH + kvh) * 2 * BLK;
-    const int tok0 = (kb * KB) % KV_PAGE;
+    const uint8_t *kc = kblk + tok0 * (D / 2), *ksc = kblk + KV_PAGE * (D / 2) + tok0 * NB;
 #pragma unroll
     for (int kt = 0; kt < 2; ++kt) {
-      const int tok = tok0 + kt * 16 + c;
-      const uint8_t* kp = kblk + tok * (D / 2) + g * (D / 8);
+      const uint8_t* kp = kc + (k_off + kt * 16 * (D / 2));
       if constexpr (D == 128) *reinterpret_cast<u32x4*>(kcode[kt]) = *reinterpret_cast<const u32x4*>(kp);
       else if constexpr (D == 64) *reinterpret_cast<uint2*>(kcode[kt]) = *reinterpret_cast<const uint2*>(kp);
       else kcode[kt][0] = *reinterpret_cast<const uint32_t*>(kp);
-      kscale[kt] = kblk[KV_PAGE * (D / 2) + tok * NB + g * NB / 4];
+      kscale[kt] = ksc[ks_off + kt * 16 * NB];
     }
-    const uint8_t* vblk = kblk + BLK;
 #pragma unroll
     for (int it = 0; it < VPASS; ++it) {
-      const int tok = tok0 + (VP <= KB ? it * VP + lane / VL : min(lane, KB - 1)), part = lane % VL;
-      vcode[it] = *reinterpret_cast<const u32x4*>(vblk + tok * (D / 2) + part * 16);
-      vscale[it] = vblk[KV_PAGE * (D / 2) + tok * NB + part];
+      vcode[it] = *reinterpret_cast<const u32x4*>(kc + BLK + (v_off + it * VP * (D / 2)));
+      vscale[it] = (ksc + BLK)[vs_off + it * VP * NB];
     }
   };
   auto page_of = [&](int kb) { return kb < b_hi ? bt[kb >> 1] : -1; };
@@ -422,7 +426,11 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   {
     const bf16_t* qp = a.q + qrow * a.q_stride + (int64_t)head * D + g * (D / 4);
 #pragma unroll
-    for (int kk = 0; kk < KS; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(qp + kk * 8);
+    for (int kk = 0; kk < KS; ++kk) {
+      u32x4 t = *reinterpret_cast<const u32x4*>(qp + kk * 8);
+      if (a.scale < 0.f) t ^= 0x80008000u;      // the largest product is then the largest score for either sign of the scale
+      qf[kk] = *reinterpret_cast<bf16x8*>(&t);
+    }
   }
   f32x4 o[D / 16];
 #pragma unroll
@@ -431,7 +439,7 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   int nan_key[NB];                               // first key whose V block is NaN, per 32-dim block
 #pragma unroll
   for (int i = 0; i < NB; ++i) nan_key[i] = INT32_MAX;
-  const float sl = a.scale * 1.4426950408889634f;   // scores in units of log2
+  const float sl = fabsf(a.scale) * 1.4426950408889634f;   // scores in units of log2
   unsigned char* sv = s_v[wave];
   const unsigned char* vr = sv + (g * 4 + (c >> 2)) * VROW + (c & 3) * 8;
 
@@ -479,31 +487,30 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
       const int kb_cur = kb;
       if (kb + NW < b_hi) fetch(kb + NW, next_page);
       // ---- softmax: lane (c, g) holds keys kt * 16 + g * 4 + j of column c
-      float t[8], mx = -FLT_MAX;
-      const bool full = kb_cur * KB + KB <= all_see;
-      if (full) {
+      float t[8], mx = -INFINITY;
+      const bool part = kb_cur * KB + KB > all_see;
+      const int lim = vis - kb_cur * KB - g * 4;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          t[i] = sacc[i >> 2][i & 3] * sl;
-          mx = fmaxf(mx, t[i]);
-        }
-      } else {
+      for (int i = 0; i < 8; ++i) t[i] = sacc[i >> 2][i & 3];
+      if (part) {       // an unseen key's score is minus infinity whatever its K holds
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          t[i] = sacc[i >> 2][i & 3] * sl;
-          if (kb_cur * KB + (i >> 2) * 16 + g * 4 + (i & 3) < vis) mx = fmaxf(mx, t[i]);
-        }
+        for (int i = 0; i < 8; ++i)
+          if (!((i >> 2) * 16 + (i & 3) < lim)) t[i] = -INFINITY;
       }
-      mx = max_swap32(max_swap16(mx));
-      const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
-      float ps = 0.f;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const bool see = full || kb_cur * KB + (i >> 2) * 16 + g * 4 + (i & 3) < vis;
-        t[i] = see ? __builtin_amdgcn_exp2f(t[i] - mn) : 0.f;
-        ps += t[i];
+      for (int i = 0; i < 8; ++i) mx = fmaxf(mx, t[i]);
+      mx = max_swap32(max_swap16(mx)) * sl;
+      // the reference m moves only when a score exceeds it by 2^8: O is seldom rescaled, weights up to 256 lose nothing.  (mx is
+      // NaN for minus infinity times a scale of 0: no key seen, m stays.)
+      const float mn = mx > m + 8.f ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f(fmaf(t[i], sl, -mn));
+      if (part && sl == 0.f) {      // (0 times minus infinity)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (!((i >> 2) * 16 + (i & 3) < lim)) t[i] = 0.f;
       }
-      l = l * corr + ps;
+      l = l * corr + (((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7])));
       m = mn;
       u32x4 ph, pl;
 #pragma unroll
@@ -669,23 +676,29 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
 
   u32x4 code[PPT];
   uint32_t scale[PPT], vtok = 0;                            // vtok: the V scales of token `lane`
-  auto fetch = [&](int pg, int page) {
+  uint32_t c_off[PPT], s_off[PPT];                          // this thread's pieces: 32-bit offsets from the page's scalar base
+#pragma unroll
+  for (int i = 0; i < PPT; ++i) {
+    const int pc = min(tid + i * NT, PIECES - 1), isv = pc >= PIECES / 2, j = pc % (PIECES / 2);
+    c_off[i] = isv * BLK + j * 16;
+    s_off[i] = isv * BLK + KV_PAGE * (D / 2) + j;
+  }
+  const uint32_t t_off = BLK + KV_PAGE * (D / 2) + lane * NB;
+  auto fetch = [&](int page) {
     const int p = page >= 0 && page < a.c.n_pages ? page : 0;
     const uint8_t* blk = a.c.pool + ((int64_t)p * KVH + kvh) * 2 * BLK;
 #pragma unroll
     for (int i = 0; i < PPT; ++i) {
-      const int pc = min(tid + i * NT, PIECES - 1), isv = pc >= PIECES / 2, j = pc % (PIECES / 2);
-      code[i] = *reinterpret_cast<const u32x4*>(blk + isv * BLK + j * 16);
-      scale[i] = blk[isv * BLK + KV_PAGE * (D / 2) + j];
+      code[i] = *reinterpret_cast<const u32x4*>(blk + c_off[i]);
+      scale[i] = blk[s_off[i]];
     }
-    const uint8_t* vs = blk + BLK + KV_PAGE * (D / 2) + lane * NB;
-    if constexpr (NB == 4) vtok = *reinterpret_cast<const uint32_t*>(vs);
-    else if constexpr (NB == 2) vtok = *reinterpret_cast<const uint16_t*>(vs);
-    else vtok = *vs;
+    if constexpr (NB == 4) vtok = *reinterpret_cast<const uint32_t*>(blk + t_off);
+    else if constexpr (NB == 2) vtok = *reinterpret_cast<const uint16_t*>(blk + t_off);
+    else vtok = blk[t_off];
   };
 
   int pg = p_lo, page = pg < p_hi ? bt[pg] : -1, next_page = pg + 1 < p_hi ? bt[pg + 1] : -1;
-  if (pg < p_hi) fetch(pg, page);
+  if (pg < p_hi) fetch(page);
   __syncthreads();                                          // s_nan
   for (int it = 0; pg < p_hi; ++pg, it ^= 1) {
     const bool there = page >= 0 && page < a.c.n_pages;
@@ -731,7 +744,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
       }
     }
     __syncthreads();      // the page is staged; and every wave is done with the page before the previous one (same buffer)
-    if (pg + 1 < p_hi) fetch(pg + 1, next_page);
+    if (pg + 1 < p_hi) fetch(next_page);
     if (there && pg * KV_PAGE < any_see) {
       // V^T fragments of 16 keys: lanes 4 r .. 4 r + 3 of a 16-lane group name row (key) r; lane i of the group gets dim i of
       // the 4 rows.  The first are requested before the scores, the others a product ahead.
@@ -952,7 +965,8 @@ static bool kv4_wide(int max_q, int H, int KVH) { return (int64_t)max_q * (H / K
 // two of 4 pages; 1 x 4k at 96 columns: 21 us in ranges of 4 pages, 26 in ranges of 8).
 int kv4_attn_splits(int n_seqs, int max_q, int max_kv, int H, int KVH) {
   const bool wide = kv4_wide(max_q, H, KVH);
-  const int tc = wide ? KV4_WIDE_TILE : KV4_NARROW_TILE, pages = max_kv / KV_PAGE;
+  const int tc = wide ? KV4_WIDE_TILE : KV4_NARROW_TILE, pages = (max_kv + KV_PAGE - 1) / KV_PAGE;
+  if (pages < 20) return 1;      // the merge is a second launch, 3 us of the host's time: not for the last microsecond
   const int64_t tiles = std::max<int64_t>(1, (int64_t)n_seqs * KVH * (((int64_t)max_q * (H / KVH) + tc - 1) / tc));
   int64_t want = (wide ? 512 : 256) / tiles;
   if (!wide && tiles >= 128 && 512 / tiles * 32 <= pages) want = 512 / tiles;

@@ -44,6 +44,7 @@ struct Kv4ReadArgs {
 int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s);
 
 constexpr int KV4_MAX_SPLITS = 256;
+constexpr int KV4_SINGLE_PAGES = 12;   // tiles of fewer pages are never split, whatever `splits` says
 
 struct Kv4AttnArgs {
   Kv4Cache c;

@@ -8,6 +8,7 @@ captured into a HIP graph; there is no CPU fallback.
 """
 from __future__ import annotations
 
+import functools
 import math
 import struct
 from typing import Optional, Tuple
@@ -25,11 +26,24 @@ _CACHE = struct.Struct("@PPiiiii")              # fmi_kv4_cache
 _ROWS = struct.Struct("@PPPqqqPqiPPdPiiiPPi")   # fmi_kv4_rows
 _QUERY = struct.Struct("@PqiPPiiiifi")          # fmi_kv4_query
 _BF16, _I32 = torch.bfloat16, torch.int32
+_raw_stream, _current_device = torch._C._cuda_getCurrentRawStream, torch._C._cuda_getDevice
 
 
 def page_bytes(n_kv_head: int, head_dim: int) -> int:
     """Bytes one page of 64 tokens takes in the pool of one layer."""
     n = _lib.load().fmi_kv4_page_bytes(int(n_kv_head), int(head_dim))
+    if n < 0:
+        check(int(n))
+    return int(n)
+
+
+@functools.lru_cache(maxsize=1024)
+def _attention_ws_bytes(n_kv_head: int, head_dim: int, n_head: int, n_seqs: int, rows: int, max_q: int, max_kv: int,
+                        splits: int) -> int:
+    """fmi_kv4_attention_ws_bytes: a function of these sizes alone"""
+    c = _CACHE.pack(0, 0, 1, n_kv_head, head_dim, n_seqs, 1)
+    q = _QUERY.pack(0, 0, n_head, 0, 0, n_seqs, rows, max_q, max_kv, 1.0, splits)
+    n = _lib.load().fmi_kv4_attention_ws_bytes(c, q)
     if n < 0:
         check(int(n))
     return int(n)
@@ -62,27 +76,24 @@ class KV4Cache:
         self.n_pages, self.n_kv_head = int(pool.shape[0]), int(pool.shape[1])
         self._dev = pool.get_device()
 
-    # ---- argument checks
+    # ---- argument checks (ordered for the calls that pass: a handful of attribute reads each)
     def _index(self, name: str, t: torch.Tensor, n: int) -> int:
         """-> the address of a contiguous int32 vector of n entries"""
-        if t.dtype is not _I32 or t.get_device() != self._dev or t.dim() != 1 or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous 1-d int32 tensor on {self.device}")
-        if t.shape[0] != n:
-            raise ValueError(f"{name} has {t.shape[0]} entries, expected {n}")
+        if t.dtype is not _I32 or t.get_device() != self._dev or not t.is_contiguous() or t.shape != (n,):
+            raise ValueError(f"{name} must be a contiguous int32 tensor ({n},) on {self.device}, not {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
         return t.data_ptr()
 
     def _rows(self, name: str, t: torch.Tensor, rows: int, heads: int) -> int:
         """-> the row stride of a bf16 tensor (rows, heads, head_dim) whose rows are contiguous"""
         D = self.head_dim
-        if t.dtype is not _BF16 or t.get_device() != self._dev or t.dim() != 3:
-            raise ValueError(f"{name} must be a bfloat16 tensor (rows, heads, {D}) on {self.device}")
-        r, h, d = t.shape
-        if r != rows or h != heads or d != D:
-            raise ValueError(f"{name} has shape {(r, h, d)}, expected {(rows, heads, D)}")
+        if t.dtype is not _BF16 or t.get_device() != self._dev or t.shape != (rows, heads, D):
+            raise ValueError(f"{name} must be a bfloat16 tensor {(rows, heads, D)} on {self.device}, not {t.dtype} "
+                             f"{tuple(t.shape)} on {t.device}")
         s0, s1, s2 = t.stride()
-        if r and (s2 != 1 or (s1 != D and h != 1)):
+        if rows and (s2 != 1 or (s1 != D and heads != 1)):
             raise ValueError(f"{name}: the heads of a row must be contiguous (strides {(s0, s1, s2)})")
-        return s0 if r > 1 else h * D
+        return s0 if rows > 1 else heads * D
 
     def _cache(self, block_table: torch.Tensor) -> bytes:
         if (block_table.dtype is not _I32 or block_table.get_device() != self._dev or block_table.dim() != 2
@@ -93,11 +104,12 @@ class KV4Cache:
 
     def _call(self, fn, *args):
         """fn(*args, stream) with the cache's device current"""
-        if torch.cuda.current_device() == self._dev:
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(self._dev))
+        dev = self._dev
+        if _current_device() == dev:
+            rc = fn(*args, _raw_stream(dev))
         else:
-            with torch.cuda.device(self._dev):
-                rc = fn(*args, torch._C._cuda_getCurrentRawStream(self._dev))
+            with torch.cuda.device(dev):
+                rc = fn(*args, _raw_stream(dev))
         if rc:
             check(rc)
 
@@ -126,8 +138,10 @@ class KV4Cache:
             heads = q.shape[1] if q.dim() == 3 else 0
             qs, qp = self._rows("q", q, rows, heads), q.data_ptr()
             if q_out is None:
-                q_out = torch.empty(rows, heads, self.head_dim, dtype=_BF16, device=self.device)
-            os, op = self._rows("q_out", q_out, rows, heads), q_out.data_ptr()
+                q_out, os = torch.empty((rows, heads, self.head_dim), dtype=_BF16, device=self.device), heads * self.head_dim
+            else:
+                os = self._rows("q_out", q_out, rows, heads)
+            op = q_out.data_ptr()
         elif q_norm is not None or q_out is not None:
             raise ValueError("q_norm and q_out go with q")
         if rope is not None:
@@ -146,7 +160,7 @@ class KV4Cache:
         return q_out
 
     def _weight(self, name: str, w: torch.Tensor) -> int:
-        if w.dtype is not _BF16 or w.get_device() != self._dev or tuple(w.shape) != (self.head_dim,) or not w.is_contiguous():
+        if w.dtype is not _BF16 or w.get_device() != self._dev or w.shape != (self.head_dim,) or not w.is_contiguous():
             raise ValueError(f"{name} must be a contiguous bfloat16 tensor ({self.head_dim},) on {self.device}")
         return w.data_ptr()
 
@@ -166,26 +180,26 @@ class KV4Cache:
         n_seqs = block_table.shape[0]
         sp, lp = self._index("q_start", q_start, n_seqs + 1), self._index("kv_len", kv_len, n_seqs)
         if out is None:
-            out = torch.empty(n, heads, self.head_dim, dtype=_BF16, device=self.device)
-        os = self._rows("out", out, n, heads)
+            out, os = torch.empty((n, heads, self.head_dim), dtype=_BF16, device=self.device), heads * self.head_dim
+        else:
+            os = self._rows("out", out, n, heads)
         if scale is None:
             scale = 1.0 / math.sqrt(self.head_dim)
         a = _QUERY.pack(q.data_ptr(), qs, heads, sp, lp, n_seqs, n, max_q, max_kv, scale, splits)
-        need = self.lib.fmi_kv4_attention_ws_bytes(c, a)
-        ws = None
-        if need > 0:       # from torch's allocator: ordered with the stream, private to a graph that is being captured
+        need = _attention_ws_bytes(self.n_kv_head, self.head_dim, heads, n_seqs, n, max_q, max_kv, splits)
+        if need:           # from torch's allocator: ordered with the stream, private to a graph that is being captured
             ws = torch.empty(need, dtype=torch.uint8, device=self.device)
-        elif need < 0:
-            check(need)
-        self._call(self.lib.fmi_op_kv4_attention, c, a, out.data_ptr(), os, ws.data_ptr() if need else 0, need)
+            self._call(self.lib.fmi_op_kv4_attention, c, a, out.data_ptr(), os, ws.data_ptr(), need)
+        else:
+            self._call(self.lib.fmi_op_kv4_attention, c, a, out.data_ptr(), os, 0, 0)
         return out
 
     def read(self, row_seq: torch.Tensor, row_pos: torch.Tensor, block_table: torch.Tensor
              ) -> Tuple[torch.Tensor, torch.Tensor]:
         """The stored values of (sequence, position) pairs: k, v bf16 (rows, n_kv_head, head_dim), exact.  Pairs outside
         the sequences, the block table or the pool read as 0."""
-        rows = row_seq.shape[0] if row_seq.dim() == 1 else -1
+        rows = row_seq.numel()
         sp, pp = self._index("row_seq", row_seq, rows), self._index("row_pos", row_pos, rows)
-        k, v = torch.empty(2, rows, self.n_kv_head, self.head_dim, dtype=_BF16, device=self.device).unbind(0)
+        k, v = torch.empty((2, rows, self.n_kv_head, self.head_dim), dtype=_BF16, device=self.device).unbind(0)
         self._call(self.lib.fmi_op_kv4_read, self._cache(block_table), sp, pp, rows, k.data_ptr(), v.data_ptr())
         return k, v
