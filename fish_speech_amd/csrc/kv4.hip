@@ -249,26 +249,37 @@ int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
 // read-back
 // =====================================================================================
 
-// the append's arrangement: a wave takes 64 / (D / 8) rows of one head of K or V, a lane 8 dims
-template <int D>
+// the append's arrangement: a wave takes 64 / (D / 8) rows, a lane 8 dims, and HC of the 2 n_kv_head blocks of K and V of a
+// page, whose codes are all requested before the first is unpacked: a row's three dependent lookups (indices, page, codes)
+// are paid once for HC blocks (32 768 rows of 8 heads: 36 us, one block per wave 55)
+template <int D, int HC>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadArgs a) {
   constexpr int LPH = D / 8, RPW = 64 / LPH, BLK = kv4_block_bytes(D);
   const int lane = threadIdx.x & 63, sub = lane % LPH;
-  const int isv = blockIdx.x & 1, kh = blockIdx.x >> 1;
+  const int hb0 = blockIdx.x * HC, blocks = 2 * a.c.KVH;
   const int64_t row = (((int64_t)blockIdx.z * 65535 + blockIdx.y) * 4 + (threadIdx.x >> 6)) * RPW + lane / LPH;
   if (row >= a.rows) return;
   const int seq = a.row_seq ? a.row_seq[row] : a.seq0, pos = a.row_seq ? a.row_pos[row] : (int)row;
-  u32x4 x = {0, 0, 0, 0};
-  if (seq >= 0 && seq < a.c.n_slots && pos >= 0 && pos < (int64_t)a.c.max_pages * KV_PAGE) {
-    const int page = a.c.block_table[(int64_t)seq * a.c.max_pages + pos / KV_PAGE];
-    if (page >= 0 && page < a.c.n_pages) {
-      const int tok = pos % KV_PAGE;
-      const uint8_t* blk = a.c.pool + (((int64_t)page * a.c.KVH + kh) * 2 + isv) * BLK;
-      const uint32_t codes = *reinterpret_cast<const uint32_t*>(blk + tok * (D / 2) + sub * 4);
-      x = kv4_unpack8(codes, kv4_scale(blk[KV_PAGE * (D / 2) + tok * (D / 32) + sub / 4]));
-    }
+  int page = -1;
+  if (seq >= 0 && seq < a.c.n_slots && pos >= 0 && pos < a.c.max_pages * KV_PAGE)
+    page = a.c.block_table[(int64_t)seq * a.c.max_pages + pos / KV_PAGE];
+  const bool there = page >= 0 && page < a.c.n_pages;
+  uint32_t code[HC], scale[HC];
+  const uint8_t* base = a.c.pool + ((there ? (int64_t)page : 0) * blocks + hb0) * BLK;
+  const int tok = there ? pos % KV_PAGE : 0, c_off = tok * (D / 2) + sub * 4, s_off = KV_PAGE * (D / 2) + tok * (D / 32) + sub / 4;
+#pragma unroll
+  for (int i = 0; i < HC; ++i) {
+    const int64_t o = (int64_t)min(i, blocks - 1 - hb0) * BLK;
+    code[i] = *reinterpret_cast<const uint32_t*>(base + o + c_off);
+    scale[i] = base[o + s_off];
   }
-  *reinterpret_cast<u32x4*>((isv ? a.v : a.k) + (row * a.c.KVH + kh) * D + sub * 8) = x;
+#pragma unroll
+  for (int i = 0; i < HC; ++i) {
+    const int hb = hb0 + i;
+    if (hb >= blocks) break;
+    const u32x4 x = kv4_unpack8(there ? code[i] : 0u, kv4_scale(there ? scale[i] : 127u));
+    *reinterpret_cast<u32x4*>((hb & 1 ? a.v : a.k) + (row * a.c.KVH + (hb >> 1)) * D + sub * 8) = x;
+  }
 }
 
 int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s) {
@@ -279,10 +290,17 @@ int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s) {
   FMI_REQUIRE(!a.row_seq == !a.row_pos, "kv4 read: null row indices");
   FMI_CHECK(kv4_check_rows("k", a.k, (int64_t)a.c.KVH * D, a.c.KVH, D));
   FMI_CHECK(kv4_check_rows("v", a.v, (int64_t)a.c.KVH * D, a.c.KVH, D));
-  const dim3 grid = kv4_row_grid(2 * (int64_t)a.c.KVH, a.rows, 4 * (64 / (D / 8)));
-  if (D == 128) hipLaunchKernelGGL((kv4_read_kernel<128>), grid, dim3(256), 0, s, a);
-  else if (D == 64) hipLaunchKernelGGL((kv4_read_kernel<64>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((kv4_read_kernel<32>), grid, dim3(256), 0, s, a);
+  const bool many = (int64_t)a.rows * a.c.KVH * D > (int64_t)1 << 21;
+  const dim3 grid = kv4_row_grid((2 * a.c.KVH + (many ? 7 : 0)) / (many ? 8 : 1), a.rows, 4 * (64 / (D / 8)));
+#define FMI_KV4_READ(D_)                                                                              \
+  do {                                                                                                \
+    if (many) hipLaunchKernelGGL((kv4_read_kernel<D_, 8>), grid, dim3(256), 0, s, a);                 \
+    else hipLaunchKernelGGL((kv4_read_kernel<D_, 1>), grid, dim3(256), 0, s, a);                      \
+  } while (0)
+  if (D == 128) FMI_KV4_READ(128);
+  else if (D == 64) FMI_KV4_READ(64);
+  else FMI_KV4_READ(32);
+#undef FMI_KV4_READ
   FMI_CHECK_HIP(hipGetLastError());
   return FMI_OK;
 }
