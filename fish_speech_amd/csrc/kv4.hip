@@ -983,7 +983,7 @@ static bool kv4_wide(int max_q, int H, int KVH) { return (int64_t)max_q * (H / K
 // two of 4 pages; 1 x 4k at 96 columns: 21 us in ranges of 4 pages, 26 in ranges of 8).
 int kv4_attn_splits(int n_seqs, int max_q, int max_kv, int H, int KVH) {
   const bool wide = kv4_wide(max_q, H, KVH);
-  const int tc = wide ? KV4_WIDE_TILE : KV4_NARROW_TILE, pages = (max_kv + KV_PAGE - 1) / KV_PAGE;
+  const int tc = wide ? KV4_WIDE_TILE : KV4_NARROW_TILE, pages = max_kv / KV_PAGE + (max_kv % KV_PAGE != 0);
   if (pages < 20) return 1;      // the merge is a second launch, 3 us of the host's time: not for the last microsecond
   const int64_t tiles = std::max<int64_t>(1, (int64_t)n_seqs * KVH * (((int64_t)max_q * (H / KVH) + tc - 1) / tc));
   int64_t want = (wide ? 512 : 256) / tiles;
@@ -1013,9 +1013,11 @@ int launch_kv4_attn(const Kv4AttnArgs& a_, hipStream_t s) {
   const bool wide = a.form ? a.form == 2 : kv4_wide(a.max_q, a.H, a.c.KVH);
   a.tile_cols = wide ? KV4_WIDE_TILE : KV4_NARROW_TILE;
   const int64_t tiles = (cols + a.tile_cols - 1) / a.tile_cols;
-  FMI_REQUIRE(tiles * a.c.KVH < (int64_t)1 << 31 && (int64_t)a.max_q * a.H < (int64_t)1 << 31, "kv4 attention: too many query rows");
-  const dim3 grid((unsigned)(tiles * a.c.KVH), a.splits, a.n_seqs), 
-             mgrid((unsigned)(((int64_t)a.max_q * a.H + (a.splits > 16 ? 0 : 3)) / (a.splits > 16 ? 1 : 4)), a.n_seqs);
+  const int64_t merges = a.splits > 16 ? (int64_t)a.max_q * a.H : ((int64_t)a.max_q * a.H + 3) / 4;
+  // (a grid dimension counts threads in 32 bits)
+  FMI_REQUIRE((int64_t)a.max_q * a.H < (int64_t)1 << 31 && tiles * a.c.KVH < (int64_t)1 << 23 &&
+                  (a.splits == 1 || merges < (int64_t)1 << 24), "kv4 attention: too many query rows per sequence (%d)", a.max_q);
+  const dim3 grid((unsigned)(tiles * a.c.KVH), a.splits, a.n_seqs), mgrid((unsigned)merges, a.n_seqs);
 #define FMI_KV4_ATTN(D_)                                                                                       \
   do {                                                                                                         \
     if (wide) hipLaunchKernelGGL((kv4_attn_wide_kernel<D_, KV4_WIDE_TILE / 32>), grid, dim3(2 * KV4_WIDE_TILE), 0, s, a); \
@@ -1078,8 +1080,9 @@ static int kv4_splits_of(const fmi_kv4_cache* cache, const fmi_kv4_query* q) {
 }
 
 int64_t fmi_kv4_attention_ws_bytes(const fmi_kv4_cache* cache, const fmi_kv4_query* q) {
-  if (!cache || !q || cache->n_kv_head < 1 || q->n_head < 1 || q->splits < 0 || q->splits > KV4_MAX_SPLITS || q->total_q < 0 ||
-      q->max_q < 0 || q->n_seqs < 0 || q->max_kv < 0)
+  if (!cache || !q || cache->n_kv_head < 1 || q->n_head < 1 || q->n_head > (1 << 16) || q->splits < 0 ||
+      q->splits > KV4_MAX_SPLITS || q->total_q < 0 || q->max_q < 0 || q->n_seqs < 0 || q->max_kv < 0 ||
+      (int64_t)q->total_q * q->n_head >= (int64_t)1 << 40)
     return set_error(FMI_EINVAL, "kv4 attention: bad sizes");
   return 4 * kv4_attn_part_floats(q->total_q, q->n_head, cache->head_dim, kv4_splits_of(cache, q));
 }

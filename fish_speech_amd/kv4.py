@@ -102,6 +102,10 @@ class KV4Cache:
         n, w = block_table.shape
         return _CACHE.pack(self.pool.data_ptr(), block_table.data_ptr(), self.n_pages, self.n_kv_head, self.head_dim, n, w)
 
+    def _new(self, rows: int, heads: int) -> torch.Tensor:
+        D = self.head_dim      # (torch.empty without strides takes a third longer)
+        return torch.empty_strided((rows, heads, D), (heads * D, D, 1), dtype=_BF16, device=self.device)
+
     def _call(self, fn, *args):
         """fn(*args, stream) with the cache's device current"""
         dev = self._dev
@@ -138,7 +142,7 @@ class KV4Cache:
             heads = q.shape[1] if q.dim() == 3 else 0
             qs, qp = self._rows("q", q, rows, heads), q.data_ptr()
             if q_out is None:
-                q_out, os = torch.empty((rows, heads, self.head_dim), dtype=_BF16, device=self.device), heads * self.head_dim
+                q_out, os = self._new(rows, heads), heads * self.head_dim
             else:
                 os = self._rows("q_out", q_out, rows, heads)
             op = q_out.data_ptr()
@@ -180,7 +184,7 @@ class KV4Cache:
         n_seqs = block_table.shape[0]
         sp, lp = self._index("q_start", q_start, n_seqs + 1), self._index("kv_len", kv_len, n_seqs)
         if out is None:
-            out, os = torch.empty((n, heads, self.head_dim), dtype=_BF16, device=self.device), heads * self.head_dim
+            out, os = self._new(n, heads), heads * self.head_dim
         else:
             os = self._rows("out", out, n, heads)
         if scale is None:
@@ -200,6 +204,6 @@ class KV4Cache:
         the sequences, the block table or the pool read as 0."""
         rows = row_seq.numel()
         sp, pp = self._index("row_seq", row_seq, rows), self._index("row_pos", row_pos, rows)
-        k, v = torch.empty((2, rows, self.n_kv_head, self.head_dim), dtype=_BF16, device=self.device).unbind(0)
+        k, v = self._new(rows, self.n_kv_head), self._new(rows, self.n_kv_head)
         self._call(self.lib.fmi_op_kv4_read, self._cache(block_table), sp, pp, rows, k.data_ptr(), v.data_ptr())
         return k, v

@@ -119,7 +119,7 @@ def test_append_refusals(bad):
 @pytest.mark.parametrize("bad", [
     dict(q_dev=None), dict(q_dev=A + 8), dict(q_stride=252), dict(q_stride=192), dict(n_head=0), dict(n_head=3), dict(q_start_dev=None),
     dict(kv_len_dev=None), dict(n_seqs=-1), dict(n_seqs=4), dict(n_seqs=65536), dict(total_q=-1), dict(max_q=-1), dict(max_kv=-1),
-    dict(splits=-1), dict(splits=257)], ids=str)
+    dict(splits=-1), dict(splits=257), dict(max_q=1 << 30), dict(max_q=1 << 26, splits=3)], ids=str)
 def test_attention_refusals(bad):
     lib = _lib.load()
     c, q = _cache(), _query(**bad)

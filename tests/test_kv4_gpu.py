@@ -399,6 +399,39 @@ def test_offsets_beyond_32_bits():
     assert cache.pool[: n_pages - 31].count_nonzero() == 0
 
 
+def test_more_rows_than_a_grid_dimension_and_values_beyond_32_bits():
+    """1.1 million rows, nearly all of them padding: q and its output pass 2^31 elements, the groups of rows pass 65 535."""
+    D, H, KVH, M = 128, 16, 1, 1_100_000
+    table = torch.tensor([[2, 0, 1]], dtype=I32, device=DEV)
+    cache = make_cache(3, KVH, D, fill=0x11)
+    rows = [0, 5, 700_001, 1_048_577, M - 1]
+    pos = torch.full((M,), -1, dtype=I32, device=DEV)
+    pos[rows] = torch.tensor([3, 190, 64, 70, 127], dtype=I32, device=DEV)
+    seq = torch.zeros(M, dtype=I32, device=DEV)
+    q = torch.zeros(M, H, D, dtype=BF, device=DEV)
+    k, v = (torch.zeros(M, KVH, D, dtype=BF, device=DEV) for _ in range(2))
+    q[rows], k[rows], v[rows] = (x.to(DEV) for x in (randn(5, H, D, seed=1), randn(5, KVH, D, seed=2), randn(5, KVH, D, seed=3)))
+    rope = rope_table(192, D)
+    out = torch.full_like(q, 7.0)
+    cache.append(k, v, seq, pos, table, q=q, q_out=out, rope=rope.to(DEV))
+    cs = rope[pos[rows].long().cpu()]
+    assert same(out[rows], O.rotate(q[rows].cpu(), cs, False))
+    out[rows] = 7.0
+    assert out.eq(7.0).all()
+    gk, gv = cache.read(seq, pos, table)
+    assert same(gk[rows], O.stored(O.rotate(k[rows].cpu(), cs, False))) and same(gv[rows], O.stored(v[rows].cpu()))
+    gk[rows] = 0
+    gv[rows] = 0
+    assert not gk.any() and not gv.any()
+    # attention rows at the end of the same buffer
+    start, n = torch.tensor([M - 2, M], dtype=I32, device=DEV), torch.tensor([128], dtype=I32, device=DEV)
+    cache.attend(q, start, n, table, max_q=2, max_kv=128, out=out)
+    ks, vs = (x.double().cpu() for x in cache.read(torch.zeros(128, dtype=I32, device=DEV),
+                                                   torch.arange(128, dtype=I32, device=DEV), table))
+    check_attention(out[-2:], q[-2:].cpu(), [(ks, vs)], [2], D)
+    assert out[:M - 2].eq(7.0).all()
+
+
 def test_a_conversation_prompt_steps_and_a_second_chunk():
     """The three operators as a generation loop uses them: a ragged prompt, single tokens, another chunk on top."""
     D, H, KVH = 64, 8, 4
