@@ -208,10 +208,10 @@ static dim3 kv4_row_grid(int64_t heads, int rows, int per) {
 }
 
 int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
-  FMI_CHECK(kv4_check_cache(a.c));
-  const int D = a.c.D;
   FMI_REQUIRE(a.rows >= 0, "kv4 append: negative row count");
   if (a.rows == 0) return FMI_OK;
+  FMI_CHECK(kv4_check_cache(a.c));
+  const int D = a.c.D;
   FMI_CHECK(kv4_check_rows("k", a.k, a.k_stride, a.c.KVH, D));
   FMI_CHECK(kv4_check_rows("v", a.v, a.v_stride, a.c.KVH, D));
   FMI_REQUIRE(a.row_seq && (a.row_pos || a.slot_pos), "kv4 append: null row indices");
@@ -219,6 +219,8 @@ int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
     FMI_REQUIRE(a.H >= 1 && a.H <= (1 << 16), "kv4 append: q of %d query heads (1 to 2^16)", a.H);
     FMI_CHECK(kv4_check_rows("q", a.q, a.q_stride, a.H, D));
     FMI_CHECK(kv4_check_rows("q_out", a.q_out, a.q_out_stride, a.H, D));
+    FMI_REQUIRE(a.q_out != a.q || (a.q_out_stride == a.q_stride && !(a.rope && a.half)),
+                "kv4 append: q_out over q needs the same row stride and no half-split rotation");
   } else {
     FMI_REQUIRE(a.H == 0 && !a.q_norm, "kv4 append: query heads or q_norm without q");
   }
@@ -283,9 +285,9 @@ __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadArgs a) {
 }
 
 int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s) {
-  FMI_CHECK(kv4_check_cache(a.c));
   FMI_REQUIRE(a.rows >= 0, "kv4 read: negative row count");
   if (a.rows == 0) return FMI_OK;
+  FMI_CHECK(kv4_check_cache(a.c));
   const int D = a.c.D;
   FMI_REQUIRE(!a.row_seq == !a.row_pos, "kv4 read: null row indices");
   FMI_CHECK(kv4_check_rows("k", a.k, (int64_t)a.c.KVH * D, a.c.KVH, D));
@@ -315,22 +317,23 @@ int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s) {
 // Keys that a column may not see enter neither the maximum nor the sum nor, where their V is NaN, the product: such blocks
 // are read as 0 and the columns that do see them are set to NaN at the end.
 struct Kv4Span {       // one sequence's query rows and keys, clamped to what the buffers hold
-  int slot, row0, nq, kv, cached;
+  int slot, row0, nq, pos0, cached;   // pos0: position of the first query row (negative: sees nothing)
 };
 __device__ inline Kv4Span kv4_span(const Kv4AttnArgs& a, int s) {
   Kv4Span r;
   r.slot = a.seq_slot ? a.seq_slot[s] : s;
   const int lo = a.q_start ? a.q_start[s] : s, hi = a.q_start ? a.q_start[s + 1] : s + 1;
   r.row0 = min(max(lo, 0), a.total_q);
-  r.nq = min(max(min(hi, a.total_q) - r.row0, 0), a.max_q);
-  r.kv = min(max(a.kv_len ? a.kv_len[s] : a.slot_pos[r.slot] + 1, 0), 1 << 30);
-  r.cached = (int)min((int64_t)r.kv, (int64_t)a.c.max_pages * KV_PAGE);
+  const int n = max(min(hi, a.total_q) - r.row0, 0), kv = min(max(a.kv_len ? a.kv_len[s] : a.slot_pos[r.slot] + 1, 0), 1 << 30);
+  r.nq = min(n, a.max_q);
+  r.pos0 = kv - n;
+  r.cached = (int)min((int64_t)kv, (int64_t)a.c.max_pages * KV_PAGE);
   return r;
 }
 
 // pages of 64 keys that the tile of `tile_cols` columns from col0 sees
 __device__ inline int kv4_tile_pages(const Kv4Span& sp, int G, int col0, int tile_cols) {
-  const int nk = min(sp.kv - sp.nq + min(col0 + tile_cols - 1, sp.nq * G - 1) / G + 1, sp.cached);
+  const int nk = min(sp.pos0 + min(col0 + tile_cols - 1, sp.nq * G - 1) / G + 1, sp.cached);
   return nk > 0 ? (nk + KV_PAGE - 1) / KV_PAGE : 0;
 }
 // the ranges a tile of np pages really uses: a function of the tile alone.  One range: its work-group writes the output itself
@@ -370,6 +373,17 @@ __device__ inline float sum_swap16(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
+// 8 values of q.  Negated for a negative scale: the largest product is then the largest score.  With an infinity among them the
+// scores are infinite or NaN and the row's softmax NaN; as NaNs from the start they cannot all be minus infinity, which would
+// pass for a row without keys.
+__device__ inline void kv4_prepare_q(u32x4& t, float scale) {
+  if (scale < 0.f) t ^= 0x80008000u;
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, max(t[i] & 0x7fffu, (t[i] >> 16) & 0x7fffu));
+  if (top >= 0x7f80u) t = (u32x4){0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+}
+
 // ---- few query columns: tiles of 16, the kernel of single tokens.  NW waves; wave w takes the 32-key blocks w, w + NW, ...
 // of the range.  Per block:
 //   scores   S^T = K Q^T, v_mfma_f32_16x16x32_bf16: lane (c, g) holds the D / 4 dims from g D / 4 of key c, which is one
@@ -399,13 +413,12 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   const Kv4Span sp = kv4_span(a, blockIdx.z);
   const int cols = sp.nq * G, col0 = tile * 16;
   if (col0 >= cols) return;
-  const int pos0 = sp.kv - sp.nq;                // position of the sequence's first query row (negative: sees nothing)
   const int np = kv4_tile_pages(sp, G, col0, 16), nz = kv4_attn_ranges(a, np);
   if (z >= nz) return;
   const int col = min(col0 + c, cols - 1);
   const int qrow = sp.row0 + col / G, head = kvh * G + col % G;
-  const int vis = min(pos0 + col / G + 1, sp.cached);          // keys [0, vis) are this column's
-  const int all_see = min(pos0 + col0 / G + 1, sp.cached);     // keys that every column of the tile sees
+  const int vis = min(sp.pos0 + col / G + 1, sp.cached);          // keys [0, vis) are this column's
+  const int all_see = min(sp.pos0 + col0 / G + 1, sp.cached);     // keys that every column of the tile sees
   const int b_lo = (int)((int64_t)z * np / nz) * 2, b_hi = (int)((int64_t)(z + 1) * np / nz) * 2;
   const int32_t* bt = a.c.block_table + (int64_t)sp.slot * a.c.max_pages;
 
@@ -446,7 +459,7 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) {
       u32x4 t = *reinterpret_cast<const u32x4*>(qp + kk * 8);
-      if (a.scale < 0.f) t ^= 0x80008000u;      // the largest product is then the largest score for either sign of the scale
+      kv4_prepare_q(t, a.scale);
       qf[kk] = *reinterpret_cast<bf16x8*>(&t);
     }
   }
@@ -594,7 +607,7 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
       O += s_o[w * SO + cc * D + d] * wgt;
       bad = min(bad, s_nan[w][d / 32]);
     }
-    if (bad < min(pos0 + row + 1, sp.cached)) O = __uint_as_float(0x7fc00000u);
+    if (bad < min(sp.pos0 + row + 1, sp.cached)) O = __uint_as_float(0x7fc00000u);
     if (nz == 1) {
       a.out[(sp.row0 + row) * a.out_stride + (int64_t)hd * D + d] = L != 0.f ? f2bf(O / L) : (bf16_t)0;
     } else {
@@ -659,17 +672,17 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   const int cols = sp.nq * G, tiles = (cols + TC - 1) / TC;
   const int tile = tiles - 1 - (int)(blockIdx.x / KVH);
   if (tile < 0) return;
-  const int col0 = tile * TC, pos0 = sp.kv - sp.nq;
+  const int col0 = tile * TC;
   const int np = kv4_tile_pages(sp, G, col0, TC), nz = kv4_attn_ranges(a, np);
   if (z >= nz) return;
   const int p_lo = (int)((int64_t)z * np / nz), p_hi = (int)((int64_t)(z + 1) * np / nz);
   const int wcol = col0 + 32 * wave;                        // this wave's first column
   const int col = min(wcol + c, cols - 1);
   const int qrow = sp.row0 + col / G, head = kvh * G + col % G;
-  const int vis = min(pos0 + col / G + 1, sp.cached);       // keys [0, vis) are this column's
+  const int vis = min(sp.pos0 + col / G + 1, sp.cached);       // keys [0, vis) are this column's
   // keys that all / any of the wave's columns see (a wave behind the last column sees none)
-  const int all_see = min(pos0 + min(wcol, cols - 1) / G + 1, sp.cached);
-  const int any_see = wcol < cols ? min(pos0 + min(wcol + 31, cols - 1) / G + 1, sp.cached) : 0;
+  const int all_see = min(sp.pos0 + min(wcol, cols - 1) / G + 1, sp.cached);
+  const int any_see = wcol < cols ? min(sp.pos0 + min(wcol + 31, cols - 1) / G + 1, sp.cached) : 0;
   const int32_t* bt = a.c.block_table + (int64_t)sp.slot * a.c.max_pages;
 
   if (tid < NB) s_nan[tid] = INT32_MAX;
@@ -679,7 +692,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       u32x4 t = *reinterpret_cast<const u32x4*>(qp + kk * 16);
-      if (a.scale < 0.f) t ^= 0x80008000u;      // the largest product is then the largest score for either sign of the scale
+      kv4_prepare_q(t, a.scale);
       qf[kk] = *reinterpret_cast<bf16x8*>(&t);
     }
   }
@@ -999,12 +1012,13 @@ int64_t kv4_attn_part_floats(int total_q, int H, int D, int splits) {
 
 int launch_kv4_attn(const Kv4AttnArgs& a_, hipStream_t s) {
   Kv4AttnArgs a = a_;
-  FMI_CHECK(kv4_check_cache(a.c));
   const int D = a.c.D;
-  FMI_REQUIRE(a.H >= 1 && a.H <= (1 << 16) && a.H % a.c.KVH == 0, "kv4 attention: %d query heads over %d kv heads", a.H, a.c.KVH);
   FMI_REQUIRE(a.n_seqs >= 0 && a.n_seqs <= 65535 && a.total_q >= 0 && a.max_q >= 0 && a.max_kv >= 0,
               "kv4 attention: bad sizes (n_seqs %d, total_q %d, max_q %d, max_kv %d)", a.n_seqs, a.total_q, a.max_q, a.max_kv);
   if (a.n_seqs == 0 || a.total_q == 0 || a.max_q == 0) return FMI_OK;
+  FMI_CHECK(kv4_check_cache(a.c));
+  FMI_REQUIRE(a.H >= 1 && a.H <= (1 << 16) && a.H % a.c.KVH == 0, "kv4 attention: %d query heads over %d kv heads", a.H, a.c.KVH);
+  FMI_REQUIRE(isfinite(a.scale), "kv4 attention: scale %g", (double)a.scale);
   FMI_CHECK(kv4_check_rows("q", a.q, a.q_stride, a.H, D));
   FMI_CHECK(kv4_check_rows("out", a.out, a.out_stride, a.H, D));
   FMI_REQUIRE(a.seq_slot || a.n_seqs <= a.c.n_slots, "kv4 attention: %d sequences, block table of %d", a.n_seqs, a.c.n_slots);

@@ -175,7 +175,7 @@ class KV4Cache:
         ``q_start[s] .. q_start[s + 1] - 1`` as its last positions and ``kv_len[s]`` cached keys, its own included;
         both int32 on the device, so a captured graph replays with new lengths.  ``max_q`` / ``max_kv``: upper bounds of
         one sequence's rows and keys (rows beyond ``max_q`` are not computed; ``max_kv`` only tunes the launch).  Rows
-        that see no key give 0.  Rows behind the last sequence are left as they were in ``out`` (undefined without one).
+        that see no key give 0, rows whose q holds an infinity or a NaN give NaN.  Rows behind the last sequence are left as they were in ``out`` (undefined without one).
         ``splits``: key ranges per query tile, 0 = chosen from the sizes; with a fixed number (and ``max_q``) a row's bits
         do not depend on the other sequences of the call."""
         n, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0

@@ -294,7 +294,7 @@ int64_t fmi_kv4_page_bytes(int n_kv_head, int head_dim);
 typedef struct fmi_kv4_rows {
   const void *q_dev, *k_dev, *v_dev;   /* q_dev NULL: keys and values only */
   int64_t q_stride, k_stride, v_stride;
-  void* q_out_dev;                     /* bf16, may be q_dev itself only if no half-split rotation is asked for */
+  void* q_out_dev;                     /* bf16, may be q_dev itself with the same stride and no half-split rotation */
   int64_t q_out_stride;
   int32_t n_head;
   const void *q_norm_dev, *k_norm_dev;
@@ -314,8 +314,8 @@ int fmi_op_kv4_read(const fmi_kv4_cache* cache, const int32_t* row_seq_dev, cons
 /* Causal attention over the cache (F.scaled_dot_product_attention, llama.py:928-934): sequence s has the query rows
  * q_start_dev[s] .. q_start_dev[s + 1] - 1 (int32 [n_seqs + 1], ascending) at its last positions, row i of n at position
  * kv_len_dev[s] - n + i, and sees the cached keys up to its own position; kv head = head / (n_head / n_kv_head).  fp32
- * scores, softmax and sums, one rounding to bf16.  A row that sees no key gives 0; rows past the last sequence stay as
- * they were.  max_q and max_kv bound the rows and keys of any sequence (they size the launch; rows beyond max_q of a
+ * scores, softmax and sums, one rounding to bf16.  A row that sees no key gives 0, one whose q holds an infinity or a NaN
+ * gives NaN; rows past the last sequence stay as they were.  scale is finite, of either sign.  max_q and max_kv bound the rows and keys of any sequence (they size the launch; rows beyond max_q of a
  * sequence are not computed).  splits: key ranges a query tile is divided into, 1 .. 256, or 0 for a choice made from
  * n_seqs, max_q and max_kv alone; with a fixed value (and max_q) a row's bits do not depend on the other sequences of the
  * call.  Up to 64 query columns (max_q times heads per kv head) the softmax weights enter the product with 16 significant

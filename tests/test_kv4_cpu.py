@@ -111,7 +111,7 @@ def test_every_entry_point_refuses_a_bad_cache(bad):
     dict(q_out_dev=None), dict(q_out_dev=A + 4), dict(q_stride=128), dict(q_out_stride=250), dict(n_head=0), dict(n_head=-4),
     dict(row_seq_dev=None), dict(row_pos_dev=None), dict(rows=-1), dict(rope_dim=0), dict(rope_dim=8), dict(rope_dim=24),
     dict(rope_dim=80), dict(rope_len=0), dict(rope_dev=A + 4), dict(q_norm_dev=A + 2), dict(k_norm_dev=A + 8),
-    dict(q_dev=None, q_norm_dev=A)], ids=str)
+    dict(q_dev=None, q_norm_dev=A), dict(rope_half=1), dict(q_out_stride=264)], ids=str)    # (q_out is q itself here)
 def test_append_refusals(bad):
     assert _lib.load().fmi_op_kv4_append(_cache(), _rows(**bad), None) == -1
 
@@ -119,7 +119,7 @@ def test_append_refusals(bad):
 @pytest.mark.parametrize("bad", [
     dict(q_dev=None), dict(q_dev=A + 8), dict(q_stride=252), dict(q_stride=192), dict(n_head=0), dict(n_head=3), dict(q_start_dev=None),
     dict(kv_len_dev=None), dict(n_seqs=-1), dict(n_seqs=4), dict(n_seqs=65536), dict(total_q=-1), dict(max_q=-1), dict(max_kv=-1),
-    dict(splits=-1), dict(splits=257), dict(max_q=1 << 30), dict(max_q=1 << 26, splits=3)], ids=str)
+    dict(scale=math.inf), dict(scale=-math.inf), dict(scale=math.nan), dict(splits=-1), dict(splits=257), dict(max_q=1 << 30), dict(max_q=1 << 26, splits=3)], ids=str)
 def test_attention_refusals(bad):
     lib = _lib.load()
     c, q = _cache(), _query(**bad)
@@ -152,8 +152,11 @@ def test_null_arguments_and_empty_calls():
     assert lib.fmi_op_kv4_append(_cache(), _rows(rows=0), None) == 0
     assert lib.fmi_op_kv4_read(_cache(), None, None, 0, None, None, None) == 0
     assert lib.fmi_op_kv4_attention(_cache(), _query(total_q=0), A, 256, None, 0, None) == 0
-    assert lib.fmi_op_kv4_attention(_cache(), _query(n_seqs=0, q_start_dev=None, kv_len_dev=None), A, 256,
-                                    None, 0, None) == 0
+    none = _cache(n_seqs=0, block_table_dev=None)
+    for c in (_cache(), none):
+        assert lib.fmi_op_kv4_attention(c, _query(n_seqs=0, q_start_dev=None, kv_len_dev=None), A, 256, None, 0, None) == 0
+    assert lib.fmi_op_kv4_append(none, _rows(rows=0), None) == 0
+    assert lib.fmi_op_kv4_read(none, None, None, 0, None, None, None) == 0
 
 
 def test_page_bytes():

@@ -368,6 +368,40 @@ def test_rows_behind_the_last_sequence_and_beyond_max_q_stay():
         check_attention(out[3:5, :H], q[3:5], kv[1:], [2], D)
 
 
+@pytest.mark.parametrize("H, n, max_q", [(4, 5, 2), (8, 90, 40)])
+def test_rows_up_to_max_q_keep_their_positions(H, n, max_q):
+    """A sequence with more rows than max_q: the first max_q are at the positions they have in the whole call."""
+    D, KVH, keys = 64, 2, [150]
+    cache, t, q, qd, start, kv_len, kv = setup_attention(D, H, KVH, [n], keys, seed=13)
+    for splits in (1, 3):
+        out = torch.full((n, H, D), 3.0, dtype=BF, device=DEV)
+        cache.attend(qd, start, kv_len, t, max_q=max_q, max_kv=150, out=out, splits=splits)
+        seen = keys[0] - n + max_q
+        check_attention(out[:max_q], q[:max_q], [(kv[0][0][:seen], kv[0][1][:seen])], [max_q], D)
+        assert out[max_q:].eq(3).all()
+
+
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+@pytest.mark.parametrize("n, splits", [(3, 1), (3, 2), (70, 1), (70, 2)])
+def test_nonfinite_queries_give_nan_where_they_see_a_key(bad, n, splits):
+    """Also if every key's score would be minus infinity; the other rows and heads do not notice."""
+    D, H, KVH, keys = 64, 4, 2, 800
+    cache, t, q, qd, start, kv_len, kv = setup_attention(D, H, KVH, [n, 2], [keys, 1], seed=17)
+    pos = torch.arange(keys, dtype=I32)
+    k = torch.ones(keys, KVH, D, dtype=BF)                         # no zero, one sign: inf times k is the same infinity for every key
+    v = randn(keys, KVH, D, seed=19)
+    cache.append(k.to(DEV), v.to(DEV), torch.zeros(keys, dtype=I32, device=DEV), pos.to(DEV), t)
+    qd[0, 1, 7], qd[2, 3, 63], qd[n, 0, 0], qd[n + 1, 2, 32] = bad, bad, bad, bad     # (row n: the 2-row sequence's row without a key)
+    got = cache.attend(qd, start, kv_len, t, max_q=n, max_kv=keys, splits=splits)
+    nan = torch.zeros(n + 2, H, dtype=torch.bool)
+    nan[0, 1] = nan[2, 3] = nan[n + 1, 2] = True
+    assert torch.equal(got.isnan().any(-1).cpu(), nan) and torch.equal(got.isnan().all(-1).cpu(), nan)
+    assert got[n].eq(0).all()
+    ref, bound = O.attend(q[:n], O.stored(k), O.stored(v), keys - n, 1 / math.sqrt(D), weight=2.0 ** -16 if n == 3 else 2.0 ** -11)
+    err = (got[:n].double().cpu() - ref).abs()
+    assert bool((err <= 2.0 ** -8 * ref.abs() + bound)[~nan[:n]].all())
+
+
 def test_rows_do_not_depend_on_their_batch_with_fixed_splits():
     D, H, KVH = 128, 32, 8
     keys, new = [700, 64, 333, 1500], [1, 1, 1, 1]
@@ -516,3 +550,8 @@ def test_empty_calls():
     s = torch.zeros(2, dtype=I32, device=DEV)
     out = cache.attend(torch.empty(0, 4, 64, dtype=BF, device=DEV), s, s[:1], t, max_q=0, max_kv=0)
     assert out.shape == (0, 4, 64)
+    # no sequences at all: every row is one behind the last
+    none, q = torch.empty(0, 2, dtype=I32, device=DEV), torch.ones(3, 4, 64, dtype=BF, device=DEV)
+    assert cache.append(z, z, e, e, none) is None
+    out = torch.full((3, 4, 64), 5.0, dtype=BF, device=DEV)
+    assert cache.attend(q, s[:1], e, none, max_q=3, max_kv=5000, out=out) is out and out.eq(5).all()
