@@ -71,6 +71,9 @@ __device__ inline float kv4_rstd(double m) {
 // is fixed by the definition (sum of squares in fp64, reciprocal norm and both products rounded to fp32, value to bf16;
 // products of the rotation are exact in fp32, one rounding of their sum, then bf16), so the stored codes do not depend on
 // how the lanes are arranged or on fused products.
+// Bound by memory for prompts: 16 384 tokens of 32 + 8 + 8 heads x 128 dims (12 288 bytes read, 8 192 of q and 1 088 of codes
+// written per token) take 67 to 74 us, 4.8 to 5.3 TB/s where a copy reaches 5.2.  One head per wave instead of eight: 108 us.
+// Few tokens are bound by the launch (8 tokens: 2.2 to 3.4 us) and better off with every head in a wave of its own.
 template <int D, bool HALF, int HC>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
   constexpr int LPH = D / 8, RPW = 64 / LPH, BLK = kv4_block_bytes(D);
@@ -253,7 +256,8 @@ int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
 
 // the append's arrangement: a wave takes 64 / (D / 8) rows, a lane 8 dims, and HC of the 2 n_kv_head blocks of K and V of a
 // page, whose codes are all requested before the first is unpacked: a row's three dependent lookups (indices, page, codes)
-// are paid once for HC blocks (32 768 rows of 8 heads: 36 us, one block per wave 55)
+// are paid once for HC blocks (32 768 rows of 8 heads, one launch after the other: 38 us = 4.5 TB/s, one block per wave 55;
+// 130 rows: 2.7 us, the launch)
 template <int D, int HC>
 __global__ __launch_bounds__(256) void kv4_read_kernel(Kv4ReadArgs a) {
   constexpr int LPH = D / 8, RPW = 64 / LPH, BLK = kv4_block_bytes(D);
@@ -393,7 +397,10 @@ __device__ inline void kv4_prepare_q(u32x4& t, float scale) {
 //   output   O^T += V^T P: V is unpacked to bf16 into the wave's LDS rows and read back transposed by
 //            ds_read_b64_tr_b16 (4 keys of one dim per lane).
 // The next block's codes are in flight during a block's arithmetic.  The waves' (m, l, O) are merged through LDS in wave
-// order.
+// order.  Bound by memory once the card is full: 64 x 8k keys of 8 kv heads x 128 dims 110 us = 5.2 TB/s, 64 x 16k 202 us =
+// 5.65; 32 sequences of 4k to 8k keys 50 us = 4.3 TB/s (the longest sequences' work-groups run on alone at the end); 1 x 128k
+// 36 us = 3.9 TB/s (the merge is 4 us of it).  One sequence of 300 keys is 5 to 6.5 us of dependent loads (lengths, page,
+// codes) and two blocks of arithmetic.  Of 4, 8 and 16 waves, 8 were the fastest.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   constexpr int KB = 32, NT = 64 * NW, BLK = kv4_block_bytes(D), NB = D / 32;
@@ -632,6 +639,9 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
 // one dword load and a maximum per wave): values are exact down to 2^-23 of the largest block's power, and what falls below
 // is under 2^-24 of the largest value, the size of the rounding of the fp32 sums.  When E grows, O is scaled down like
 // with a growing maximum.
+// Bound by issue: per page and wave 32 matrix instructions (34 % of the time) and 260 others (43 %), two waves per SIMD to
+// overlap them.  8 prompts of 2k tokens over 4k keys run at 960 TFLOP/s, two ragged ones at 850 (222 us; the last
+// work-groups run alone), 8 ragged prompts of up to 200 tokens in 14.5 us, mostly the latency of their 1 to 4 pages.
 // The native product of 4-bit K with Q in two 8-bit parts needs no unpacking and the same matrix time, but its sums came out
 // 9e-5 of the absolute sum away from the exact ones (bf16 products: 1e-7), too coarse for scores.
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
@@ -907,7 +917,8 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
 // joins the key ranges of a query row and head: D / 4 lanes per range, WPR waves (1, or 4 for more than 16 ranges) per row
 // and head, the ranges dealt over the groups of D / 4 lanes and their sums joined in group order.  grid (rows and heads of
 // the longest sequence, 4 / WPR to a work-group; n_seqs).  A group's first ranges are requested before the weights are
-// known: the two loads of a range wait for each other no more than once.
+// known: the two loads of a range wait for each other no more than once.  2.4 to 3.4 us for 8 rows x 32 heads x 4 ranges, 3.8
+// to 4.6 for 1 x 32 x 32: a launch and its latency.
 template <int D, int WPR>
 __global__ __launch_bounds__(256) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
   constexpr int LN = D / 4, NG = 64 * WPR / LN, PRE = WPR == 1 ? 16 / NG : 4;
@@ -989,8 +1000,10 @@ constexpr int KV4_NARROW_COLS = 64, KV4_NARROW_TILE = 16, KV4_WIDE_TILE = 128;
 static bool kv4_wide(int max_q, int H, int KVH) { return (int64_t)max_q * (H / KVH) > KV4_NARROW_COLS; }
 
 // Enough work-groups to fill the 256 CUs, no more: a range costs its work-group's start and a partial state.
-// Narrow: one work-group per CU (8 x 2k keys: 256 work-groups 11.4 us, 512 13.0); two where ranges of 32 pages remain, for
-// sequences of different lengths (32 ragged x 8k: 48 us for 512, 54 for 256; 32 x 4k: 36 for 512, 32 for 256).
+// Narrow: one work-group per CU (8 x 2k keys: 256 work-groups 12.0 us, 512 12.9); two where ranges of 32 pages remain, for
+// sequences of different lengths (32 ragged x 8k: 54 us for 512, 60 for 256; 32 x 4k: 36 for 512, 32 for 256).  Equal shares of
+// all pages instead, cut without regard to sequences, were slower throughout (32 ragged x 8k 60 us, 8 x 2k 19): a share
+// that crosses a border pays a second start and merge.
 // Wide: two fit a CU (8 x 4k keys at 128 columns: 49 us for 256 work-groups, 42 for 512, 52 for 1024), with ranges of at
 // least 8 pages where more than 128 rows would write partial states (32 x 500 keys at 128 columns: 24 us in one range, 50 in
 // two of 4 pages; 1 x 4k at 96 columns: 21 us in ranges of 4 pages, 26 in ranges of 8).

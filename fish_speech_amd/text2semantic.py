@@ -168,7 +168,8 @@ def init_model(checkpoint_path, device, precision=torch.bfloat16, compile: bool 
 
 def launch_thread_safe_queue(checkpoint_path, device, precision=torch.bfloat16, compile: bool = False, kv_bits: int = 16):
     """One worker thread owns the model and serves GenerateRequests from the returned queue; `None` stops it
-    (inference.py:748-799).  ``kv_bits=4`` keeps the K/V cache in 4-bit floats.  Errors travel back as WrappedGenerateResponse("error", exception)."""
+    (inference.py:748-799).  Errors travel back as WrappedGenerateResponse("error", exception).  ``kv_bits=4`` keeps the
+    K/V cache in 4-bit floats (MiDualAR.setup_caches)."""
     input_queue: queue.Queue = queue.Queue()
     ready = threading.Event()
     failure: List[BaseException] = []
