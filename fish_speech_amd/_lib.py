@@ -93,6 +93,7 @@ _SIGS = {
     "fmi_op_kv4_read": (C.c_int, [_P, _P, _P, _I, _P, _P, _P]),
     "fmi_kv4_attention_ws_bytes": (C.c_int64, [_P, _P]),
     "fmi_op_kv4_attention": (C.c_int, [_P, _P, _P, C.c_int64, _P, C.c_int64, _P]),
+    "fmi_op_kv4_step": (C.c_int, [_P, _P, C.c_float, _I, _I, _P, C.c_int64, _P, C.c_int64, _P]),
     "fmi_dac_arena_bytes": (C.c_int64, [C.POINTER(DacConfigC)]),
     "fmi_dac_create": (C.c_int, [C.POINTER(DacConfigC), _P, C.c_int64, C.POINTER(_P)]),
     "fmi_dac_destroy": (None, [_P]),

@@ -365,34 +365,39 @@ int block_slow_rest(fmi_dualar* h, const LayerW& w, bf16_t* x, int rows, hipStre
   return FMI_OK;
 }
 
-// K/V append and attention over the 4-bit cache: ws.qkv -> ws.ao.  The key ranges of a decode step are a function of the
-// row's own position (kv4_attn_ranges under a fixed KV4_SPLITS); prompts run in one range and always on the wide tiles, also
-// the few rows of a resumed one: an utterance's numbers do not depend on its batch-mates or on how its prompt was cut.
+// K/V append and attention over the 4-bit cache: ws.qkv -> ws.ao, one launch for a decode step.  The key ranges of a step are a
+// function of the row's own position (kv4_attn_ranges under a fixed KV4_SPLITS); prompts run in one range and always on the
+// wide tiles, also the few rows of a resumed one: an utterance's numbers do not depend on its batch-mates or on how its prompt
+// was cut.
 constexpr int KV4_SPLITS = 16;
 int attn_kv4(fmi_dualar* h, const LayerW& w, int layer, int rows, const int32_t* row_slot, const int32_t* row_pos, hipStream_t s) {
   const Dims& d = h->slow;
   Workspace& ws = h->ws;
-  const Kv4Cache c{h->kv4_pool[layer], h->st.block_table, h->n_pages, d.KVH, d.D, h->max_batch, h->max_pages};
   Kv4AppendArgs p{};
-  p.c = c; p.q = ws.qkv; p.k = ws.qkv + d.H * d.D; p.v = ws.qkv + (d.H + d.KVH) * d.D;
-  p.q_stride = p.k_stride = p.v_stride = d.qkv; p.q_out = ws.q; p.q_out_stride = d.H * d.D; p.H = d.H;
+  p.c = Kv4Cache{h->kv4_pool[layer], h->st.block_table, h->n_pages, d.KVH, d.D, h->max_batch, h->max_pages};
+  p.q = ws.qkv; p.k = ws.qkv + d.H * d.D; p.v = ws.qkv + (d.H + d.KVH) * d.D;
+  p.q_stride = p.k_stride = p.v_stride = d.qkv; p.H = d.H;
   p.q_norm = h->cfg.attention_qk_norm ? w.q_norm : nullptr;
   p.k_norm = h->cfg.attention_qk_norm ? w.k_norm : nullptr;
   p.eps = h->cfg.norm_eps; p.rope = h->rope; p.rope_len = h->cfg.max_seq_len; p.rot = d.D;
-  p.row_seq = row_slot; p.row_pos = row_pos; p.slot_pos = h->st.pos; p.slot_done = row_pos ? nullptr : h->st.done; p.rows = rows;
-  FMI_CHECK(launch_kv4_append(p, s));
+  p.row_seq = row_slot; p.rows = rows;
   Kv4AttnArgs a{};
-  a.c = c; a.q = ws.q; a.out = ws.ao; a.q_stride = a.out_stride = d.H * d.D; a.slot_pos = h->st.pos; a.total_q = rows;
-  a.max_kv = h->max_seq; a.H = d.H; a.scale = 1.0f / sqrtf((float)d.D);
-  if (row_pos) {
-    a.q_start = h->kv4_seq; a.kv_len = h->kv4_seq + h->max_batch + 1; a.seq_slot = h->kv4_seq + 2 * h->max_batch + 1;
-    a.n_seqs = h->kv4_n; a.max_q = h->kv4_max_q; a.splits = 1; a.form = 2;
-  } else {
-    a.seq_slot = row_slot; a.n_seqs = rows; a.max_q = 1; a.form = 1; a.part = h->kv4_part;
+  a.out = ws.ao; a.out_stride = d.H * d.D; a.scale = 1.0f / sqrtf((float)d.D);
+  if (!row_pos) {
+    p.slot_pos = h->st.pos; p.slot_done = h->st.done;
+    a.part = h->kv4_part;
     a.splits = (h->attn_mask & 2) ? KV4_SPLITS : 1;   // (bit 2 unset: no row is long enough to be split, the merge launch is saved)
+    FMI_CHECK(launch_kv4_step(p, a, s));
+    h->launches += a.splits > 1 ? 2 : 1;
+    return FMI_OK;
   }
+  p.row_pos = row_pos; p.q_out = ws.q; p.q_out_stride = d.H * d.D;
+  FMI_CHECK(launch_kv4_append(p, s));
+  a.c = p.c; a.q = ws.q; a.q_stride = d.H * d.D; a.total_q = rows; a.max_kv = h->max_seq; a.H = d.H;
+  a.q_start = h->kv4_seq; a.kv_len = h->kv4_seq + h->max_batch + 1; a.seq_slot = h->kv4_seq + 2 * h->max_batch + 1;
+  a.n_seqs = h->kv4_n; a.max_q = h->kv4_max_q; a.splits = 1; a.wide = true;
   FMI_CHECK(launch_kv4_attn(a, s));
-  h->launches += a.splits > 1 ? 3 : 2;
+  h->launches += 2;
   return FMI_OK;
 }
 

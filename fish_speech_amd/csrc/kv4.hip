@@ -11,6 +11,7 @@
 #include <math.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "kv4_kernels.h"
 
@@ -65,6 +66,93 @@ __device__ inline float kv4_rstd(double m) {
   return (float)y;
 }
 
+// A lane's 8 dims of a head: the norm weights and rotation factors that belong to them.  HALF: the rotation pairs dims rot / 2
+// apart, so the other element of each pair is in another chunk, `xp`, which the lane reads and norms too.
+template <int D, bool HALF>
+struct Kv4Chunk {
+  float wv[8], wp[8], cs[8], sn[8];
+
+  __device__ inline void load_norm(const bf16_t* nw, int sub, int psub) {
+    const u32x4 w0 = *reinterpret_cast<const u32x4*>(nw + sub * 8), w1 = *reinterpret_cast<const u32x4*>(nw + psub * 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      wv[i] = i & 1 ? bf_hi(w0[i >> 1]) : bf_lo(w0[i >> 1]);
+      if (HALF) wp[i] = i & 1 ? bf_hi(w1[i >> 1]) : bf_lo(w1[i >> 1]);
+    }
+  }
+  // pos_tab: the position's rot / 2 (cos, sin).  Interleaved: cs / sn [i] of pair i (i < 4); half: of this lane's element i, the
+  // sine negated for the first of a pair
+  __device__ inline void load_rope(const bf16_t* pos_tab, int rot, int sub) {
+    const int hr = rot / 2;
+    const bool first = sub * 8 < hr;
+    const bf16_t* tab = pos_tab + (HALF ? (first ? sub * 8 : sub * 8 - hr) * 2 : sub * 8);
+    uint32_t t[8];
+    *reinterpret_cast<u32x4*>(t) = *reinterpret_cast<const u32x4*>(tab);
+    if (HALF) *reinterpret_cast<u32x4*>(t + 4) = *reinterpret_cast<const u32x4*>(tab + 8);
+#pragma unroll
+    for (int i = 0; i < (HALF ? 8 : 4); ++i) {
+      cs[i] = bf_lo(t[i]);
+      sn[i] = HALF && first ? -bf_hi(t[i]) : bf_hi(t[i]);
+    }
+  }
+  // the D / 8 lanes of a head together
+  __device__ inline void norm(u32x4& x, u32x4& xp, double eps, int lane) const {
+    double ss = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const double e0 = (double)bf_lo(x[i]), e1 = (double)bf_hi(x[i]);
+      ss = fma(e0, e0, ss);
+      ss = fma(e1, e1, ss);
+    }
+    ss += xor_lane_d<1>(ss, lane);
+    ss += xor_lane_d<2>(ss, lane);
+    if (D / 8 > 4) ss += xor_lane_d<4>(ss, lane);
+    if (D / 8 > 8) ss += xor_lane_d<8>(ss, lane);
+    const float rstd = kv4_rstd(ss * (1.0 / D) + eps);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[i] = kv4_pk_bf16(bf_lo(x[i]) * rstd * wv[2 * i], bf_hi(x[i]) * rstd * wv[2 * i + 1]);
+      if (HALF) xp[i] = kv4_pk_bf16(bf_lo(xp[i]) * rstd * wp[2 * i], bf_hi(xp[i]) * rstd * wp[2 * i + 1]);
+    }
+  }
+  __device__ inline void rotate(u32x4& x, const u32x4& xp) const {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float x0 = bf_lo(x[i]), x1 = bf_hi(x[i]);
+      if (!HALF) x[i] = kv4_pk_bf16(x0 * cs[i] - x1 * sn[i], x1 * cs[i] + x0 * sn[i]);
+      else x[i] = kv4_pk_bf16(x0 * cs[2 * i] + bf_lo(xp[i]) * sn[2 * i], x1 * cs[2 * i + 1] + bf_hi(xp[i]) * sn[2 * i + 1]);
+    }
+  }
+};
+// the chunk that holds the partners of chunk `sub`
+__device__ inline int kv4_partner(int sub, int rot) { return sub * 8 < rot / 2 ? sub + rot / 16 : sub - rot / 16; }
+
+// 8 dims -> 8 codes; 4 lanes hold a block.  -> its scale byte
+__device__ inline uint32_t kv4_quantise(const u32x4& x, int lane, uint32_t& codes) {
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) top = max(top, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
+  top = max(top, (uint32_t)xor_lane<1>((int)top, lane));
+  top = max(top, (uint32_t)xor_lane<2>((int)top, lane));
+  const bool finite = top < 0x7f80u;
+  // max = 1.f * 2^(exp - 127): the power with max <= 7 * 2^e is exp - 127 - 2, one more above f = 1.75
+  const int b = min(max((int)(top >> 7) - 2 + ((top & 0x7fu) > 0x60u ? 1 : 0), KV4_MIN_SCALE), KV4_MAX_SCALE);
+  const float sc = kv4_scale((uint32_t)b);
+  uint32_t r = 0;
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2_t, (uint32_t)x[0]), sc, 0);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2_t, (uint32_t)x[1]), sc, 1);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2_t, (uint32_t)x[2]), sc, 2);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(r, __builtin_bit_cast(bf16x2_t, (uint32_t)x[3]), sc, 3);
+  codes = finite ? r : 0u;
+  return finite ? (uint32_t)b : (uint32_t)KV4_NAN_SCALE;
+}
+// ... and into the block of a page
+template <int D>
+__device__ inline void kv4_store(uint8_t* blk, int tok, int sub, uint32_t codes, uint32_t scale) {
+  *reinterpret_cast<uint32_t*>(blk + tok * (D / 2) + sub * 4) = codes;
+  if ((sub & 3) == 0) blk[KV_PAGE * (D / 2) + tok * (D / 32) + sub / 4] = (uint8_t)scale;
+}
+
 // D / 8 lanes own one (row, head), 8 dims each; a wave takes 64 / (D / 8) consecutive rows of one head, so its code bytes are
 // consecutive in the page, and up to HC heads of one kind (q, k or v) one after the other: indices, page and rotation are
 // looked up once for them, the next head's values are in flight.  grid (chunks of heads; groups of rows).  Every rounding
@@ -89,40 +177,18 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
   const bf16_t* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + row * stride;
   const bf16_t* nw = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
   const bool rotated = kind != 2 && a.rope && sub * 8 < a.rot;
-  // half layout: the other element of each pair lies rot / 2 dims away, in another lane's chunk
-  const int hr = a.rot / 2;
-  const bool first = sub * 8 < hr;
-  const int psub = HALF && rotated ? (first ? sub + hr / 8 : sub - hr / 8) : sub;
+  const int psub = HALF && rotated ? kv4_partner(sub, a.rot) : sub;
   u32x4 nx = *reinterpret_cast<const u32x4*>(src + h0 * D + sub * 8), nxp;
   if (HALF) nxp = *reinterpret_cast<const u32x4*>(src + h0 * D + psub * 8);
   const int seq = in_rows ? a.row_seq[row] : -1;
   const bool seq_ok = seq >= 0 && seq < a.c.n_slots;
-  const int pos = seq_ok ? (a.row_pos ? a.row_pos[row] : a.slot_pos[seq]) : -1;
+  const int pos = seq_ok ? a.row_pos[row] : -1;
   const bool valid = pos >= 0 && pos < (a.rope ? min(a.c.max_pages * KV_PAGE, a.rope_len) : a.c.max_pages * KV_PAGE);
   const bool rot = rotated && valid;
-  int page = kind != 0 && valid ? a.c.block_table[(int64_t)seq * a.c.max_pages + pos / KV_PAGE] : -1;
-  if (kind != 0 && valid && a.slot_done && a.slot_done[seq]) page = -1;
-  float wv[8], wp[8], cs[8], sn[8];
-  if (nw) {
-    const u32x4 w0 = *reinterpret_cast<const u32x4*>(nw + sub * 8), w1 = *reinterpret_cast<const u32x4*>(nw + psub * 8);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      wv[i] = i & 1 ? bf_hi(w0[i >> 1]) : bf_lo(w0[i >> 1]);
-      if (HALF) wp[i] = i & 1 ? bf_hi(w1[i >> 1]) : bf_lo(w1[i >> 1]);
-    }
-  }
-  if (rot) {
-    // interleaved: cs / sn [i] of pair i (i < 4); half: of this lane's element i, the sine negated for the first of a pair
-    const bf16_t* tab = a.rope + (int64_t)pos * a.rot + (HALF ? (first ? sub * 8 : sub * 8 - hr) * 2 : sub * 8);
-    uint32_t t[8];
-    *reinterpret_cast<u32x4*>(t) = *reinterpret_cast<const u32x4*>(tab);
-    if (HALF) *reinterpret_cast<u32x4*>(t + 4) = *reinterpret_cast<const u32x4*>(tab + 8);
-#pragma unroll
-    for (int i = 0; i < (HALF ? 8 : 4); ++i) {
-      cs[i] = bf_lo(t[i]);
-      sn[i] = HALF && first ? -bf_hi(t[i]) : bf_hi(t[i]);
-    }
-  }
+  const int page = kind != 0 && valid ? a.c.block_table[(int64_t)seq * a.c.max_pages + pos / KV_PAGE] : -1;
+  Kv4Chunk<D, HALF> ch;
+  if (nw) ch.load_norm(nw, sub, psub);
+  if (rot) ch.load_rope(a.rope + (int64_t)pos * a.rot, a.rot, sub);
   const bool store = page >= 0 && page < a.c.n_pages;
   const int tok = pos % KV_PAGE;
   // (a lane without a page never uses its addresses)
@@ -134,56 +200,15 @@ __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
       nx = *reinterpret_cast<const u32x4*>(src + (h + 1) * D + sub * 8);
       if (HALF) nxp = *reinterpret_cast<const u32x4*>(src + (h + 1) * D + psub * 8);
     }
-    if (nw) {
-      double ss = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const double e0 = (double)bf_lo(x[i]), e1 = (double)bf_hi(x[i]);
-        ss = fma(e0, e0, ss);
-        ss = fma(e1, e1, ss);
-      }
-      ss += xor_lane_d<1>(ss, lane);
-      ss += xor_lane_d<2>(ss, lane);
-      if (LPH > 4) ss += xor_lane_d<4>(ss, lane);
-      if (LPH > 8) ss += xor_lane_d<8>(ss, lane);
-      const float rstd = kv4_rstd(ss * (1.0 / D) + a.eps);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[i] = kv4_pk_bf16(bf_lo(x[i]) * rstd * wv[2 * i], bf_hi(x[i]) * rstd * wv[2 * i + 1]);
-        if (HALF) xp[i] = kv4_pk_bf16(bf_lo(xp[i]) * rstd * wp[2 * i], bf_hi(xp[i]) * rstd * wp[2 * i + 1]);
-      }
-    }
-    if (rot) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float x0 = bf_lo(x[i]), x1 = bf_hi(x[i]);
-        if (!HALF) x[i] = kv4_pk_bf16(x0 * cs[i] - x1 * sn[i], x1 * cs[i] + x0 * sn[i]);
-        else x[i] = kv4_pk_bf16(x0 * cs[2 * i] + bf_lo(xp[i]) * sn[2 * i], x1 * cs[2 * i + 1] + bf_hi(xp[i]) * sn[2 * i + 1]);
-      }
-    }
+    if (nw) ch.norm(x, xp, a.eps, lane);
+    if (rot) ch.rotate(x, xp);
     if (kind == 0) {
       if (valid) *reinterpret_cast<u32x4*>(a.q_out + row * a.q_out_stride + h * D + sub * 8) = x;
       continue;
     }
-    // ---- quantise: 4 lanes hold a 32-dim block
-    uint32_t top = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, max(x[i] & 0x7fffu, (x[i] >> 16) & 0x7fffu));
-    top = max(top, (uint32_t)xor_lane<1>((int)top, lane));
-    top = max(top, (uint32_t)xor_lane<2>((int)top, lane));
-    const bool finite = top < 0x7f80u;
-    // max = 1.f * 2^(exp - 127): the power with max <= 7 * 2^e is exp - 127 - 2, one more above f = 1.75
-    const int b = min(max((int)(top >> 7) - 2 + ((top & 0x7fu) > 0x60u ? 1 : 0), KV4_MIN_SCALE), KV4_MAX_SCALE);
-    const float sc = kv4_scale((uint32_t)b);
-    uint32_t codes = 0;
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[0]), sc, 0);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[1]), sc, 1);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[2]), sc, 2);
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(codes, __builtin_bit_cast(bf16x2_t, (uint32_t)x[3]), sc, 3);
-    if (!store) continue;
-    uint8_t* hb = blk + (int64_t)h * 2 * BLK;
-    *reinterpret_cast<uint32_t*>(hb + tok * (D / 2) + sub * 4) = finite ? codes : 0u;
-    if ((sub & 3) == 0) hb[KV_PAGE * (D / 2) + tok * (D / 32) + sub / 4] = (uint8_t)(finite ? b : KV4_NAN_SCALE);
+    uint32_t codes;
+    const uint32_t scale = kv4_quantise(x, lane, codes);
+    if (store) kv4_store<D>(blk + (int64_t)h * 2 * BLK, tok, sub, codes, scale);
   }
 }
 
@@ -210,20 +235,15 @@ static dim3 kv4_row_grid(int64_t heads, int rows, int per) {
   return dim3((unsigned)heads, (unsigned)std::min<int64_t>(groups, 65535), (unsigned)((groups + 65534) / 65535));
 }
 
-int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
-  FMI_REQUIRE(a.rows >= 0, "kv4 append: negative row count");
-  if (a.rows == 0) return FMI_OK;
+static int kv4_check_append(const Kv4AppendArgs& a) {   // of an append or a step
   FMI_CHECK(kv4_check_cache(a.c));
   const int D = a.c.D;
   FMI_CHECK(kv4_check_rows("k", a.k, a.k_stride, a.c.KVH, D));
   FMI_CHECK(kv4_check_rows("v", a.v, a.v_stride, a.c.KVH, D));
-  FMI_REQUIRE(a.row_seq && (a.row_pos || a.slot_pos), "kv4 append: null row indices");
+  FMI_REQUIRE(a.row_seq, "kv4: null row sequences");
   if (a.q) {
     FMI_REQUIRE(a.H >= 1 && a.H <= (1 << 16), "kv4 append: q of %d query heads (1 to 2^16)", a.H);
     FMI_CHECK(kv4_check_rows("q", a.q, a.q_stride, a.H, D));
-    FMI_CHECK(kv4_check_rows("q_out", a.q_out, a.q_out_stride, a.H, D));
-    FMI_REQUIRE(a.q_out != a.q || (a.q_out_stride == a.q_stride && !(a.rope && a.half)),
-                "kv4 append: q_out over q needs the same row stride and no half-split rotation");
   } else {
     FMI_REQUIRE(a.H == 0 && !a.q_norm, "kv4 append: query heads or q_norm without q");
   }
@@ -231,6 +251,20 @@ int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
   if (a.rope) {
     FMI_REQUIRE(((uintptr_t)a.rope & 15) == 0 && a.rope_len >= 1, "kv4 append: empty or misaligned rotation table");
     FMI_REQUIRE(a.rot >= 16 && a.rot <= D && a.rot % 16 == 0, "kv4 append: %d rotated dims (a multiple of 16 up to head_dim %d)", a.rot, D);
+  }
+  return FMI_OK;
+}
+
+int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
+  FMI_REQUIRE(a.rows >= 0, "kv4 append: negative row count");
+  if (a.rows == 0) return FMI_OK;
+  FMI_CHECK(kv4_check_append(a));
+  FMI_REQUIRE(a.row_pos, "kv4 append: null row positions");
+  const int D = a.c.D;
+  if (a.q) {
+    FMI_CHECK(kv4_check_rows("q_out", a.q_out, a.q_out_stride, a.H, D));
+    FMI_REQUIRE(a.q_out != a.q || (a.q_out_stride == a.q_stride && !(a.rope && a.half)),
+                "kv4 append: q_out over q needs the same row stride and no half-split rotation");
   }
   const bool half = a.rope && a.half, many = (int64_t)a.rows * (a.H + 2 * a.c.KVH) * D > (int64_t)1 << 23;
   const int hc = many ? 8 : 1;
@@ -325,10 +359,19 @@ struct Kv4Span {       // one sequence's query rows and keys, clamped to what th
 };
 __device__ inline Kv4Span kv4_span(const Kv4AttnArgs& a, int s) {
   Kv4Span r;
+  if (a.step_len > 0) {      // one row, at a given position; none if that or its sequence is not there
+    const int seq = a.seq_slot[s];
+    const bool seq_ok = seq >= 0 && seq < a.c.n_slots;
+    r.slot = seq_ok ? seq : 0;
+    r.row0 = s;
+    r.pos0 = seq_ok ? (a.row_pos ? a.row_pos[s] : a.slot_pos[r.slot]) : -1;
+    r.nq = r.pos0 >= 0 && r.pos0 < a.step_len;
+    r.cached = r.pos0 + 1;
+    return r;
+  }
   r.slot = a.seq_slot ? a.seq_slot[s] : s;
-  const int lo = a.q_start ? a.q_start[s] : s, hi = a.q_start ? a.q_start[s + 1] : s + 1;
-  r.row0 = min(max(lo, 0), a.total_q);
-  const int n = max(min(hi, a.total_q) - r.row0, 0), kv = min(max(a.kv_len ? a.kv_len[s] : a.slot_pos[r.slot] + 1, 0), 1 << 30);
+  r.row0 = min(max(a.q_start[s], 0), a.total_q);
+  const int n = max(min(a.q_start[s + 1], a.total_q) - r.row0, 0), kv = min(max(a.kv_len[s], 0), 1 << 30);
   r.nq = min(n, a.max_q);
   r.pos0 = kv - n;
   r.cached = (int)min((int64_t)kv, (int64_t)a.c.max_pages * KV_PAGE);
@@ -401,8 +444,16 @@ __device__ inline void kv4_prepare_q(u32x4& t, float scale) {
 // 5.65; 32 sequences of 4k to 8k keys 50 us = 4.3 TB/s (the longest sequences' work-groups run on alone at the end); 1 x 128k
 // 36 us = 3.9 TB/s (the merge is 4 us of it).  One sequence of 300 keys is 5 to 6.5 us of dependent loads (lengths, page,
 // codes) and two blocks of arithmetic.  Of 4, 8 and 16 waves, 8 were the fastest.
-template <int D, int NW>
-__global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
+//
+// STEP 1 / 2 (rotation interleaved / half split): a generation step of one new token per sequence in the same launch.  Every
+// work-group norms and rotates its own query heads (into LDS rows); the one of a kv head's last range also quantises the new
+// token's K and V, stores them, and puts them over what it fetched of that token: nothing is read back from memory, and no
+// other work-group reads that token.  The values and their bits are those of an append followed by an attention.  In a
+// captured graph 8 x 300 keys take 8.4 us where the two launches take 9.5, 16 x 1k 12.7 and 14.3, 32 x 6k 49 and 53; a
+// model's frame of 36 layers went from 4.15 to 4.10 ms at 200 tokens, the host's part of a call pair from 17.6 to 10.2 us.
+struct Kv4None {};
+template <int D, int NW, int STEP>
+__global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::conditional_t<STEP != 0, Kv4AppendArgs, Kv4None> p) {
   constexpr int KB = 32, NT = 64 * NW, BLK = kv4_block_bytes(D), NB = D / 32;
   constexpr int KS = D / 32;                     // k-steps of a score product
   constexpr int VROW = D * 2 + 32;               // bytes of a key's row in LDS: 32 more, so that the 4 rows a 16-lane
@@ -428,6 +479,36 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   const int all_see = min(sp.pos0 + col0 / G + 1, sp.cached);     // keys that every column of the tile sees
   const int b_lo = (int)((int64_t)z * np / nz) * 2, b_hi = (int)((int64_t)(z + 1) * np / nz) * 2;
   const int32_t* bt = a.c.block_table + (int64_t)sp.slot * a.c.max_pages;
+
+  // the new token: D / 8 lanes per head, the tile's query heads, then K, then V; requested before the codes, which take longer
+  constexpr int LPH = D / 8, QROW = D * 2 + 16;
+  static_assert(NT / LPH >= 18, "16 query heads, K and V at a time");
+  __shared__ __attribute__((aligned(16))) unsigned char s_q[STEP ? 16 * QROW : 16];
+  __shared__ __attribute__((aligned(16))) uint32_t s_code[STEP ? 2 : 1][LPH];
+  __shared__ uint32_t s_scale[STEP ? 2 : 1][NB];
+  Kv4Chunk<D, STEP == 2> ch;
+  u32x4 x, xp;
+  const int item = tid / LPH, sub = tid % LPH, heads = min(16, cols - col0), newest = z == nz - 1 ? sp.pos0 / KB : -1;
+  bool normed = false, rotated = false;
+  if constexpr (STEP != 0) {
+    const int64_t row = sp.row0;
+    const bf16_t* src = p.q + row * p.q_stride + (kvh * G + col0 + min(item, heads - 1)) * D;
+    const bf16_t* nw = p.q_norm;
+    if (item == heads) {
+      src = p.k + row * p.k_stride + kvh * D;
+      nw = p.k_norm;
+    } else if (item == heads + 1) {
+      src = p.v + row * p.v_stride + kvh * D;
+      nw = nullptr;
+    }
+    normed = nw;
+    rotated = p.rope && item != heads + 1 && sub * 8 < p.rot;
+    const int psub = STEP == 2 && rotated ? kv4_partner(sub, p.rot) : sub;
+    x = *reinterpret_cast<const u32x4*>(src + sub * 8);
+    if (STEP == 2) xp = *reinterpret_cast<const u32x4*>(src + psub * 8);
+    if (normed) ch.load_norm(nw, sub, psub);
+    if (rotated) ch.load_rope(p.rope + (int64_t)sp.pos0 * p.rot, p.rot, sub);
+  }
 
   // K and V codes and scales of one block; a missing page reads page 0 and is skipped later.  A lane's place in the block is
   // fixed: 32-bit offsets from a scalar base.
@@ -460,12 +541,29 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   if (kb < b_hi) fetch(kb, page);
   int next_page = page_of(kb + NW);
 
+  if constexpr (STEP != 0) {
+    if (normed) ch.norm(x, xp, p.eps, lane);
+    if (rotated) ch.rotate(x, xp);
+    if (item < heads) *reinterpret_cast<u32x4*>(s_q + item * QROW + sub * 16) = x;
+    uint32_t codes;
+    const uint32_t scale = kv4_quantise(x, lane, codes);
+    const int kv = item - heads;
+    if (newest >= 0 && (kv == 0 || kv == 1)) {
+      s_code[kv][sub] = codes;
+      if ((sub & 3) == 0) s_scale[kv][sub / 4] = scale;
+      const int pg = bt[sp.pos0 / KV_PAGE];
+      if (pg >= 0 && pg < a.c.n_pages && !(p.slot_done && p.slot_done[sp.slot]))
+        kv4_store<D>(a.c.pool + (((int64_t)pg * KVH + kvh) * 2 + kv) * BLK, sp.pos0 % KV_PAGE, sub, codes, scale);
+    }
+    __syncthreads();
+  }
   bf16x8 qf[KS];                                 // B operand: column c, dims g D / 4 + 8 kk ..
   {
-    const bf16_t* qp = a.q + qrow * a.q_stride + (int64_t)head * D + g * (D / 4);
+    const bf16_t* qp = STEP ? nullptr : a.q + qrow * a.q_stride + (int64_t)head * D + g * (D / 4);
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) {
-      u32x4 t = *reinterpret_cast<const u32x4*>(qp + kk * 8);
+      u32x4 t = STEP ? *reinterpret_cast<const u32x4*>(s_q + min(c, heads - 1) * QROW + (g * (D / 4) + kk * 8) * 2)
+                     : *reinterpret_cast<const u32x4*>(qp + kk * 8);
       kv4_prepare_q(t, a.scale);
       qf[kk] = *reinterpret_cast<bf16x8*>(&t);
     }
@@ -484,6 +582,22 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a) {
   for (; kb < b_hi; kb += NW) {
     const bool there = page >= 0 && page < a.c.n_pages;
     if (there) {
+      if (STEP != 0 && kb == newest) {     // the new token's K and V over what the page held there
+        const int key_new = sp.pos0 % KB;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+          if (kt * 16 + c == key_new) {
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) kcode[kt][kk] = s_code[0][g * KS + kk];
+            kscale[kt] = s_scale[0][g * NB / 4];
+          }
+#pragma unroll
+        for (int it = 0; it < VPASS; ++it)
+          if (it * VP + lane / VL == key_new) {
+            vcode[it] = *reinterpret_cast<const u32x4*>(&s_code[STEP ? 1 : 0][lane % VL * 4]);
+            vscale[it] = s_scale[STEP ? 1 : 0][lane % VL];
+          }
+      }
       // ---- scores
       f32x4 sacc[2];
 #pragma unroll
@@ -1037,7 +1151,7 @@ int launch_kv4_attn(const Kv4AttnArgs& a_, hipStream_t s) {
   FMI_REQUIRE(a.seq_slot || a.n_seqs <= a.c.n_slots, "kv4 attention: %d sequences, block table of %d", a.n_seqs, a.c.n_slots);
   FMI_REQUIRE(a.splits >= 1 && a.splits <= KV4_MAX_SPLITS && (a.splits == 1 || a.part), "kv4 attention: bad split of the keys");
   const int64_t cols = (int64_t)a.max_q * (a.H / a.c.KVH);
-  const bool wide = a.form ? a.form == 2 : kv4_wide(a.max_q, a.H, a.c.KVH);
+  const bool wide = a.wide || kv4_wide(a.max_q, a.H, a.c.KVH);
   a.tile_cols = wide ? KV4_WIDE_TILE : KV4_NARROW_TILE;
   const int64_t tiles = (cols + a.tile_cols - 1) / a.tile_cols;
   const int64_t merges = a.splits > 16 ? (int64_t)a.max_q * a.H : ((int64_t)a.max_q * a.H + 3) / 4;
@@ -1048,7 +1162,7 @@ int launch_kv4_attn(const Kv4AttnArgs& a_, hipStream_t s) {
 #define FMI_KV4_ATTN(D_)                                                                                       \
   do {                                                                                                         \
     if (wide) hipLaunchKernelGGL((kv4_attn_wide_kernel<D_, KV4_WIDE_TILE / 32>), grid, dim3(2 * KV4_WIDE_TILE), 0, s, a); \
-    else hipLaunchKernelGGL((kv4_attn_kernel<D_, 8>), grid, dim3(512), 0, s, a);                               \
+    else hipLaunchKernelGGL((kv4_attn_kernel<D_, 8, 0>), grid, dim3(512), 0, s, a, Kv4None{});                 \
     if (a.splits > 16) hipLaunchKernelGGL((kv4_attn_merge_kernel<D_, 4>), mgrid, dim3(256), 0, s, a);          \
     else if (a.splits > 1) hipLaunchKernelGGL((kv4_attn_merge_kernel<D_, 1>), mgrid, dim3(256), 0, s, a);      \
   } while (0)
@@ -1056,6 +1170,37 @@ int launch_kv4_attn(const Kv4AttnArgs& a_, hipStream_t s) {
   else if (D == 64) FMI_KV4_ATTN(64);
   else FMI_KV4_ATTN(32);
 #undef FMI_KV4_ATTN
+  FMI_CHECK_HIP(hipGetLastError());
+  return FMI_OK;
+}
+
+int launch_kv4_step(const Kv4AppendArgs& p, const Kv4AttnArgs& a_, hipStream_t s) {
+  Kv4AttnArgs a = a_;
+  FMI_REQUIRE(p.rows >= 0 && p.rows <= 65535, "kv4 step: %d rows (0 to 65535)", p.rows);
+  if (p.rows == 0) return FMI_OK;
+  FMI_CHECK(kv4_check_append(p));
+  FMI_REQUIRE(p.row_pos || p.slot_pos, "kv4 step: null row positions");
+  const int D = p.c.D;
+  FMI_REQUIRE(p.q && p.H % p.c.KVH == 0, "kv4 step: %d query heads over %d kv heads", p.H, p.c.KVH);
+  FMI_CHECK(kv4_check_rows("out", a.out, a.out_stride, p.H, D));
+  FMI_REQUIRE(isfinite(a.scale), "kv4 step: scale %g", (double)a.scale);
+  FMI_REQUIRE(a.splits >= 1 && a.splits <= KV4_MAX_SPLITS && (a.splits == 1 || a.part), "kv4 step: bad split of the keys");
+  a.c = p.c; a.H = p.H; a.seq_slot = p.row_seq; a.row_pos = p.row_pos; a.slot_pos = p.slot_pos;
+  a.n_seqs = a.total_q = p.rows; a.max_q = 1; a.tile_cols = KV4_NARROW_TILE;
+  a.step_len = p.rope ? std::min(p.c.max_pages * KV_PAGE, p.rope_len) : p.c.max_pages * KV_PAGE;
+  const int tiles = (p.H / p.c.KVH + KV4_NARROW_TILE - 1) / KV4_NARROW_TILE, half = p.rope && p.half;
+  const dim3 grid((unsigned)(tiles * p.c.KVH), a.splits, p.rows), mgrid((unsigned)(a.splits > 16 ? p.H : (p.H + 3) / 4), p.rows);
+#define FMI_KV4_STEP(D_)                                                                                       \
+  do {                                                                                                         \
+    if (half) hipLaunchKernelGGL((kv4_attn_kernel<D_, 8, 2>), grid, dim3(512), 0, s, a, p);                    \
+    else hipLaunchKernelGGL((kv4_attn_kernel<D_, 8, 1>), grid, dim3(512), 0, s, a, p);                         \
+    if (a.splits > 16) hipLaunchKernelGGL((kv4_attn_merge_kernel<D_, 4>), mgrid, dim3(256), 0, s, a);          \
+    else if (a.splits > 1) hipLaunchKernelGGL((kv4_attn_merge_kernel<D_, 1>), mgrid, dim3(256), 0, s, a);      \
+  } while (0)
+  if (D == 128) FMI_KV4_STEP(128);
+  else if (D == 64) FMI_KV4_STEP(64);
+  else FMI_KV4_STEP(32);
+#undef FMI_KV4_STEP
   FMI_CHECK_HIP(hipGetLastError());
   return FMI_OK;
 }
@@ -1078,8 +1223,7 @@ int64_t fmi_kv4_page_bytes(int n_kv_head, int head_dim) {
   return (int64_t)n_kv_head * 2 * kv4_block_bytes(head_dim);
 }
 
-int fmi_op_kv4_append(const fmi_kv4_cache* cache, const fmi_kv4_rows* r, void* stream) {
-  FMI_REQUIRE(cache && r, "null argument");
+static Kv4AppendArgs kv4_append_args(const fmi_kv4_cache* cache, const fmi_kv4_rows* r) {
   Kv4AppendArgs a{};
   a.c = kv4_cache_of(*cache);
   a.q = (const bf16_t*)r->q_dev; a.k = (const bf16_t*)r->k_dev; a.v = (const bf16_t*)r->v_dev;
@@ -1088,8 +1232,12 @@ int fmi_op_kv4_append(const fmi_kv4_cache* cache, const fmi_kv4_rows* r, void* s
   a.q_norm = (const bf16_t*)r->q_norm_dev; a.k_norm = (const bf16_t*)r->k_norm_dev; a.eps = r->norm_eps;
   a.rope = (const bf16_t*)r->rope_dev; a.rope_len = r->rope_len; a.rot = r->rope_dim; a.half = r->rope_half != 0;
   a.row_seq = r->row_seq_dev; a.row_pos = r->row_pos_dev; a.rows = r->rows;
-  FMI_REQUIRE(a.rows <= 0 || a.row_pos, "kv4 append: null row positions");
-  return launch_kv4_append(a, (hipStream_t)stream);
+  return a;
+}
+
+int fmi_op_kv4_append(const fmi_kv4_cache* cache, const fmi_kv4_rows* r, void* stream) {
+  FMI_REQUIRE(cache && r, "null argument");
+  return launch_kv4_append(kv4_append_args(cache, r), (hipStream_t)stream);
 }
 
 int fmi_op_kv4_read(const fmi_kv4_cache* cache, const int32_t* row_seq_dev, const int32_t* row_pos_dev, int rows,
@@ -1128,6 +1276,22 @@ int fmi_op_kv4_attention(const fmi_kv4_cache* cache, const fmi_kv4_query* q, voi
   FMI_REQUIRE(ws_bytes >= need, "kv4 attention: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
   FMI_REQUIRE(need == 0 || (ws_dev && ((uintptr_t)ws_dev & 15) == 0), "kv4 attention: null or misaligned workspace");
   return launch_kv4_attn(a, (hipStream_t)stream);
+}
+
+int fmi_op_kv4_step(const fmi_kv4_cache* cache, const fmi_kv4_rows* r, float scale, int max_kv, int splits, void* out_dev,
+                    int64_t out_stride, void* ws_dev, int64_t ws_bytes, void* stream) {
+  FMI_REQUIRE(cache && r, "null argument");
+  const Kv4AppendArgs p = kv4_append_args(cache, r);
+  FMI_REQUIRE(!p.q_out, "kv4 step: the rotated q is not written (q_out_dev must be null)");
+  fmi_kv4_query q{};
+  q.n_head = std::max(p.H, 1); q.n_seqs = q.total_q = p.rows; q.max_q = 1; q.max_kv = max_kv; q.splits = splits;
+  const int64_t need = fmi_kv4_attention_ws_bytes(cache, &q);
+  if (need < 0) return (int)need;
+  FMI_REQUIRE(ws_bytes >= need, "kv4 step: workspace of %lld bytes, %lld needed", (long long)ws_bytes, (long long)need);
+  FMI_REQUIRE(need == 0 || (ws_dev && ((uintptr_t)ws_dev & 15) == 0), "kv4 step: null or misaligned workspace");
+  Kv4AttnArgs a{};
+  a.out = (bf16_t*)out_dev; a.out_stride = out_stride; a.scale = scale; a.splits = kv4_splits_of(cache, &q); a.part = (float*)ws_dev;
+  return launch_kv4_step(p, a, (hipStream_t)stream);
 }
 
 }  // extern "C"

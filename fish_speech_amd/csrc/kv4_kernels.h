@@ -27,9 +27,9 @@ struct Kv4AppendArgs {
   double eps;
   const bf16_t* rope;                       // [rope_len][rot / 2][2] (cos, sin) or nullptr
   int rope_len, rot, half;
-  const int32_t *row_seq, *row_pos;         // row_pos == nullptr: slot_pos[row_seq[r]]
-  const int32_t* slot_pos;
-  const int32_t* slot_done;                 // rows of a slot with a set flag do not append (nullptr: none)
+  const int32_t *row_seq, *row_pos;
+  // launch_kv4_step only: row_pos == nullptr: slot_pos[row_seq[r]]; rows of a slot with a set flag are not stored (nullptr: none)
+  const int32_t *slot_pos, *slot_done;
   int rows;
 };
 int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s);
@@ -52,19 +52,24 @@ struct Kv4AttnArgs {
   bf16_t* out;
   int64_t q_stride, out_stride;
   const int32_t* seq_slot;                  // [n_seqs] slot of each sequence, nullptr = identity
-  const int32_t* q_start;                   // [n_seqs + 1] first query row of each sequence, nullptr = one row each
-  const int32_t* kv_len;                    // [n_seqs] keys of each sequence, nullptr = slot_pos[slot] + 1
-  const int32_t* slot_pos;
+  const int32_t* q_start;                   // [n_seqs + 1] first query row of each sequence
+  const int32_t* kv_len;                    // [n_seqs] keys of each sequence
   int n_seqs, total_q, max_q, max_kv, H;
   float scale;
   int splits;                               // most key ranges per query tile (kv4_attn_splits), >= 1
   float* part;                              // splits > 1: kv4_attn_part_floats
-  int form;                                 // 0: the tile width follows max_q; 1 / 2: narrow / wide tiles, whatever max_q is
+  bool wide;                                // wide tiles whatever max_q is
   int tile_cols;                            // set by the launch: query columns per tile
+  // set by launch_kv4_step: one row per sequence seq_slot[i], at row_pos[i] (nullptr: slot_pos) if that is below step_len
+  const int32_t *row_pos, *slot_pos;
+  int step_len;
 };
 // most key ranges a call of these sizes is split into: a function of the host's sizes only
 int kv4_attn_splits(int n_seqs, int max_q, int max_kv, int H, int KVH);
 int64_t kv4_attn_part_floats(int total_q, int H, int D, int splits);
 int launch_kv4_attn(const Kv4AttnArgs& a, hipStream_t s);
+
+// append p's rows (one per sequence; q_out is not used) and attend from them; of `a`: out, out_stride, scale, splits, part
+int launch_kv4_step(const Kv4AppendArgs& p, const Kv4AttnArgs& a, hipStream_t s);
 
 }  // namespace fmi

@@ -1,4 +1,4 @@
-"""The 4-bit paged K/V cache as a Python object: append, attend, read.
+"""The 4-bit paged K/V cache as a Python object: append, attend, step (both in one launch), read.
 
 The reference's cache holds K and V in the model's own type (KVCache, fish_speech/models/text2semantic/llama.py:196-214);
 :class:`KV4Cache` holds one layer of it at 4.25 bits per value (include/fishmi.h has the number format and the pool's
@@ -131,13 +131,8 @@ class KV4Cache:
 
         Rows whose sequence or position lies outside the block table (or the rotation table) are padding: nothing is
         written for them, in the cache or in ``q_out``.  A (sequence, position) pair may appear once per call."""
-        rows, KVH = k.shape[0], self.n_kv_head
-        ks, vs = self._rows("k", k, rows, KVH), self._rows("v", v, rows, KVH)
-        ps, pp = self._index("row_seq", row_seq, rows), self._index("row_pos", row_pos, rows)
-        if rope_layout not in ("interleaved", "half"):
-            raise ValueError(f"rope_layout {rope_layout!r}: 'interleaved' or 'half'")
-        half = rope_layout == "half"
-        qp = qs = op = os = heads = qn = kn = rp = rl = rd = 0
+        qp = qs = op = os = heads = 0
+        rows = k.shape[0]
         if q is not None:
             heads = q.shape[1] if q.dim() == 3 else 0
             qs, qp = self._rows("q", q, rows, heads), q.data_ptr()
@@ -148,20 +143,31 @@ class KV4Cache:
             op = q_out.data_ptr()
         elif q_norm is not None or q_out is not None:
             raise ValueError("q_norm and q_out go with q")
+        if qp and op == qp and rope is not None and rope_layout == "half":
+            raise ValueError("the half-split rotation cannot write q_out over q")
+        a = self._new_rows(qp, qs, op, os, heads, k, v, row_seq, row_pos, rope, rope_layout, q_norm, k_norm, eps)
+        self._call(self.lib.fmi_op_kv4_append, self._cache(block_table), a)
+        return q_out
+
+    def _new_rows(self, qp, qs, op, os, heads, k, v, row_seq, row_pos, rope, rope_layout, q_norm, k_norm, eps) -> bytes:
+        """-> fmi_kv4_rows of checked arguments"""
+        rows, KVH = k.shape[0], self.n_kv_head
+        ks, vs = self._rows("k", k, rows, KVH), self._rows("v", v, rows, KVH)
+        ps, pp = self._index("row_seq", row_seq, rows), self._index("row_pos", row_pos, rows)
+        if rope_layout not in ("interleaved", "half"):
+            raise ValueError(f"rope_layout {rope_layout!r}: 'interleaved' or 'half'")
+        qn = kn = rp = rl = rd = 0
         if rope is not None:
             if (rope.dtype is not _BF16 or rope.get_device() != self._dev or rope.dim() != 3 or rope.shape[2] != 2
                     or not rope.is_contiguous()):
                 raise ValueError(f"rope must be a contiguous bfloat16 tensor (positions, dims / 2, 2) on {self.device}")
             rp, rl, rd = rope.data_ptr(), rope.shape[0], 2 * rope.shape[1]
-            if half and qp and op == qp:
-                raise ValueError("the half-split rotation cannot write q_out over q")
         if q_norm is not None:
             qn = self._weight("q_norm", q_norm)
         if k_norm is not None:
             kn = self._weight("k_norm", k_norm)
-        a = _ROWS.pack(qp, k.data_ptr(), v.data_ptr(), qs, ks, vs, op, os, heads, qn, kn, eps, rp, rl, rd, half, ps, pp, rows)
-        self._call(self.lib.fmi_op_kv4_append, self._cache(block_table), a)
-        return q_out
+        return _ROWS.pack(qp, k.data_ptr(), v.data_ptr(), qs, ks, vs, op, os, heads, qn, kn, eps, rp, rl, rd,
+                          rope_layout == "half", ps, pp, rows)
 
     def _weight(self, name: str, w: torch.Tensor) -> int:
         if w.dtype is not _BF16 or w.get_device() != self._dev or w.shape != (self.head_dim,) or not w.is_contiguous():
@@ -196,6 +202,29 @@ class KV4Cache:
             self._call(self.lib.fmi_op_kv4_attention, c, a, out.data_ptr(), os, ws.data_ptr(), need)
         else:
             self._call(self.lib.fmi_op_kv4_attention, c, a, out.data_ptr(), os, 0, 0)
+        return out
+
+    def step(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor,
+             block_table: torch.Tensor, *, max_kv: int, rope: Optional[torch.Tensor] = None, rope_layout: str = "interleaved",
+             q_norm: Optional[torch.Tensor] = None, k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6,
+             out: Optional[torch.Tensor] = None, scale: Optional[float] = None, splits: int = 0) -> torch.Tensor:
+        """A generation step, one new token per sequence, in one launch: ``append`` of the rows, then the attention of each
+        row's q over the keys up to its own position -- the same stored bytes and the same output as ``append`` and ``attend``
+        (with the same ``splits``).  A sequence may have one row per call; padding rows are left as they were in ``out``
+        (undefined without one).  The other arguments are theirs."""
+        rows, heads = k.shape[0], q.shape[1] if q.dim() == 3 else 0
+        qs = self._rows("q", q, rows, heads)
+        a = self._new_rows(q.data_ptr(), qs, 0, 0, heads, k, v, row_seq, row_pos, rope, rope_layout, q_norm, k_norm, eps)
+        if out is None:
+            out, os = self._new(rows, heads), heads * self.head_dim
+        else:
+            os = self._rows("out", out, rows, heads)
+        if scale is None:
+            scale = 1.0 / math.sqrt(self.head_dim)
+        need = _attention_ws_bytes(self.n_kv_head, self.head_dim, max(heads, 1), rows, rows, 1, max_kv, splits)
+        ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None    # (as in attend)
+        self._call(self.lib.fmi_op_kv4_step, self._cache(block_table), a, scale, max_kv, splits, out.data_ptr(), os,
+                   ws.data_ptr() if need else 0, need)
         return out
 
     def read(self, row_seq: torch.Tensor, row_pos: torch.Tensor, block_table: torch.Tensor

@@ -335,6 +335,15 @@ int64_t fmi_kv4_attention_ws_bytes(const fmi_kv4_cache* cache, const fmi_kv4_que
 int fmi_op_kv4_attention(const fmi_kv4_cache* cache, const fmi_kv4_query* query, void* out_dev, int64_t out_stride,
                          void* ws_dev, int64_t ws_bytes, void* stream);
 
+/* A generation step in one launch: fmi_op_kv4_append of `rows`, then the attention of each row's q over the keys up to its own
+ * position, with the same stored bytes and the same output bits as the two calls (one query row per sequence, up to 64
+ * heads per kv head) under the same `splits`.  q is required, q_out_dev is null; a sequence may have one row per call.  out: bf16
+ * [rows][n_head][head_dim], rows out_stride elements apart; padding rows are left as they were.  At most 65535 rows.
+ * Workspace: fmi_kv4_attention_ws_bytes of a query with n_seqs = total_q = rows, max_q = 1 and the same n_head, max_kv and
+ * splits. */
+int fmi_op_kv4_step(const fmi_kv4_cache* cache, const fmi_kv4_rows* rows, float scale, int max_kv, int splits, void* out_dev,
+                    int64_t out_stride, void* ws_dev, int64_t ws_bytes, void* stream);
+
 /* ------------------------------------------------------------------------- codec (DAC) -- */
 
 typedef struct fmi_dac fmi_dac;

@@ -103,6 +103,7 @@ def test_every_entry_point_refuses_a_bad_cache(bad):
     assert lib.fmi_op_kv4_append(c, _rows(), None) == -1
     assert lib.fmi_op_kv4_read(c, A, A, 3, A, A, None) == -1
     assert lib.fmi_op_kv4_attention(c, _query(), A, 256, None, 0, None) == -1
+    assert lib.fmi_op_kv4_step(c, _rows(q_out_dev=None), 0.1, 100, 1, A, 256, None, 0, None) == -1
     assert b"kv4" in lib.fmi_last_error()
 
 
@@ -137,6 +138,32 @@ def test_attention_refuses_a_missing_or_small_workspace_and_bad_outputs():
     assert lib.fmi_op_kv4_attention(c, q, None, 256, A, need, None) == -1
     assert lib.fmi_op_kv4_attention(c, q, A, 192, A, need, None) == -1
     assert lib.fmi_kv4_attention_ws_bytes(c, _query(splits=1)) == 0
+
+
+@pytest.mark.parametrize("bad", [
+    dict(k_dev=None), dict(v_dev=A + 2), dict(k_stride=64), dict(q_dev=None), dict(q_dev=A + 8), dict(q_stride=128), dict(q_out_dev=A),
+    dict(n_head=0), dict(n_head=3), dict(row_seq_dev=None), dict(row_pos_dev=None), dict(rows=-1), dict(rows=65536), dict(rope_dim=8),
+    dict(rope_len=0), dict(rope_dev=A + 4), dict(q_norm_dev=A + 2), dict(k_norm_dev=A + 8)], ids=str)
+def test_step_refuses_bad_rows(bad):
+    rows = _rows(**{**dict(q_out_dev=None), **bad})
+    assert _lib.load().fmi_op_kv4_step(_cache(), rows, 0.1, 100, 1, A, 256, None, 0, None) == -1
+
+
+def test_step_refuses_bad_outputs_scales_and_workspaces():
+    lib = _lib.load()
+    c, rows = _cache(), _rows(q_out_dev=None)
+    ok = dict(scale=0.1, max_kv=100, splits=1, out=A, stride=256, ws=None, ws_bytes=0)
+    need = lib.fmi_kv4_attention_ws_bytes(c, _query(n_seqs=7, total_q=7, max_q=1, splits=3))
+    assert need > 0
+    for bad in (dict(out=None), dict(out=A + 4), dict(stride=192), dict(stride=252), dict(scale=math.nan), dict(scale=math.inf),
+                dict(max_kv=-1), dict(splits=-1), dict(splits=257), dict(splits=3, ws=A, ws_bytes=need - 1),
+                dict(splits=3, ws=None, ws_bytes=need), dict(splits=3, ws=A + 4, ws_bytes=need)):
+        a = {**ok, **bad}
+        assert lib.fmi_op_kv4_step(c, rows, a["scale"], a["max_kv"], a["splits"], a["out"], a["stride"], a["ws"], a["ws_bytes"],
+                                   None) == -1, bad
+    assert lib.fmi_op_kv4_step(None, rows, 0.1, 100, 1, A, 256, None, 0, None) == -1
+    assert lib.fmi_op_kv4_step(c, None, 0.1, 100, 1, A, 256, None, 0, None) == -1
+    assert lib.fmi_op_kv4_step(c, _rows(q_out_dev=None, rows=0), 0.1, 100, 1, A, 256, None, 0, None) == 0
 
 
 def test_null_arguments_and_empty_calls():
@@ -190,6 +217,8 @@ def _call(cache, what, **kw):
     if what == "attend":
         a = dict(q=torch.zeros(3, 4, 64, dtype=bf), q_start=torch.zeros(3, dtype=i32), kv_len=torch.zeros(2, dtype=i32),
                  block_table=torch.zeros(2, 3, dtype=i32), max_q=3, max_kv=10)
+    if what == "step":
+        a.update(q=torch.zeros(3, 4, 64, dtype=bf), max_kv=10)
     if what == "read":
         a = {k: a[k] for k in ("row_seq", "row_pos", "block_table")}
     a.update(kw)
@@ -214,6 +243,10 @@ BF = torch.bfloat16
     ("attend", dict(q=torch.zeros(3, 4, 64))), ("attend", dict(q_start=torch.zeros(2, dtype=torch.int32))),
     ("attend", dict(kv_len=torch.zeros(3, dtype=torch.int32))), ("attend", dict(kv_len=torch.zeros(2, dtype=torch.int64))),
     ("attend", dict(out=torch.zeros(2, 4, 64, dtype=BF))),
+    ("step", dict(q=torch.zeros(3, 4, 64))), ("step", dict(q=torch.zeros(2, 4, 64, dtype=BF))), ("step", dict(k=torch.zeros(3, 3, 64, dtype=BF))),
+    ("step", dict(row_seq=torch.zeros(2, dtype=torch.int32))), ("step", dict(row_pos=torch.zeros(3))), ("step", dict(rope_layout="x")),
+    ("step", dict(rope=torch.zeros(9, 64, dtype=BF))), ("step", dict(k_norm=torch.zeros(32, dtype=BF))),
+    ("step", dict(out=torch.zeros(3, 5, 64, dtype=BF))), ("step", dict(block_table=torch.zeros(3, dtype=torch.int32))),
     ("read", dict(row_seq=torch.zeros(2, dtype=torch.int32))), ("read", dict(row_pos=torch.zeros(3, 1, dtype=torch.int32))),
 ])
 def test_python_argument_errors(cache, what, kw):

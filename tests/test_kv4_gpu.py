@@ -499,6 +499,138 @@ def test_a_conversation_prompt_steps_and_a_second_chunk():
     assert same(gk, torch.cat([torch.cat(a) for a, _ in hist])) and same(gv, torch.cat([torch.cat(b) for _, b in hist]))
 
 
+# ------------------------------------------------------------------------------------------------ a step in one launch
+
+
+STEP_POS = [0, 1, 31, 32, 63, 64, 65, 100, 127, 128, 300, 703, 704, 1500]
+
+
+def setup_step(D, H, KVH, pos, rot, norm, seed=0):
+    """A cache that holds the tokens before `pos` of each sequence; what it holds at and behind them reads as NaN."""
+    table, n_pages = make_table([p + 1 for p in pos], seed=seed)
+    cache = make_cache(n_pages, KVH, D, fill=0xFF)
+    k, v = randn(sum(pos), KVH, D, seed=seed + 1), randn(sum(pos), KVH, D, seed=seed + 2)
+    t, s, p, kd, vd = cuda(table, *rows_of(pos), k, v)
+    cache.append(kd, vd, s, p, t)
+    qkv = randn(len(pos), H + 2 * KVH, D, seed=seed + 3)
+    rope = rope_table(max(pos) + 1, rot) if rot else None
+    wq, wk = (randn(D, seed=seed + 4) + 1, randn(D, seed=seed + 5) + 1) if norm else (None, None)
+    return cache, t, qkv, rope, wq, wk, k, v
+
+
+def append_then_attend(cache, q, k, v, seq, pos, t, max_kv, splits, rope, layout, wq, wk, scale=None):
+    """-> the output and the pool afterwards, by the two calls on a copy of the cache; rows in the table's order"""
+    from fish_speech_amd.kv4 import KV4Cache
+
+    c = KV4Cache(cache.n_pages, cache.n_kv_head, cache.head_dim, pool=cache.pool.clone())
+    q = c.append(k, v, seq, pos, t, q=q, rope=rope, rope_layout=layout, q_norm=wq, k_norm=wk, eps=1e-5)
+    start = torch.arange(len(seq) + 1, dtype=I32, device=DEV)
+    return c.attend(q, start, pos + 1, t, max_q=1, max_kv=max_kv, splits=splits, scale=scale), c.pool
+
+
+@pytest.mark.parametrize("D, H, KVH, rot, half, norm", [
+    (128, 32, 8, 128, False, True), (128, 5, 5, 64, True, True), (128, 16, 2, 0, False, False), (64, 14, 2, 32, True, False),
+    (64, 6, 2, 64, True, True), (64, 8, 4, 16, False, True), (32, 4, 2, 32, False, True), (32, 6, 2, 16, True, False),
+    (32, 17, 1, 32, True, True), (64, 40, 1, 64, False, True), (128, 10, 2, 128, True, True)])
+@pytest.mark.parametrize("splits", [0, 1, 3, 20])
+def test_a_step_equals_append_and_attention(D, H, KVH, rot, half, norm, splits):
+    cache, t, qkv, rope, wq, wk, k0, v0 = setup_step(D, H, KVH, STEP_POS, rot, norm, seed=D + H)
+    seq, pos = torch.arange(len(STEP_POS), dtype=I32), torch.tensor(STEP_POS, dtype=I32)
+    d, s, p, r, dq, dk = cuda(qkv, seq, pos, rope, wq, wk)
+    q, k, v = d.split([H, KVH, KVH], dim=1)
+    layout = "half" if half else "interleaved"
+    want, pool = append_then_attend(cache, q, k, v, s, p, t, 1501, splits, r, layout, dq, dk)
+    got = cache.step(q, k, v, s, p, t, max_kv=1501, rope=r, rope_layout=layout, q_norm=dq, k_norm=dk, eps=1e-5, splits=splits)
+    assert torch.equal(got, want) and torch.equal(cache.pool, pool)
+    if splits == 0:
+        cs = rope[pos.long()] if rot else None
+        wantq = O.rotate(O.head_norm(qkv[:, :H], wq, 1e-5), cs, half)
+        newk = O.stored(O.rotate(O.head_norm(qkv[:, H:H + KVH], wk, 1e-5), cs, half))
+        newv = O.stored(qkv[:, H + KVH:])
+        kv = [(torch.cat([a, newk[i:i + 1]]), torch.cat([b, newv[i:i + 1]]))
+              for i, (a, b) in enumerate(zip(O.stored(k0).split(STEP_POS), O.stored(v0).split(STEP_POS)))]
+        check_attention(got, wantq, kv, [1] * len(STEP_POS), D)
+
+
+def test_a_steps_padding_rows_missing_pages_strides_and_row_order():
+    """Rows in another order than the table's sequences, rows that are padding, pages that are not there, strided rows."""
+    D, H, KVH = 64, 8, 2
+    at = [130, 64, 700, 5, 90]
+    cache, t, qkv, rope, _, _, _, _ = setup_step(D, H, KVH, at, 64, False, seed=31)
+    t = t.clone()
+    t[1, 1] = -1                                                   # sequence 1: the new token's page
+    t[2, 3] = cache.n_pages                                        # sequence 2: a page in the middle
+    rows = [(3, 5), (-1, 5), (0, 130), (5, 3), (2, 700), (4, -1), (1, 64), (4, 2 ** 31 - 1), (2 ** 31 - 1, 0), (4, 701)]
+    seq, pos = (torch.tensor([x[i] for x in rows], dtype=I32) for i in range(2))     # (the table of rotations ends at 700)
+    M = len(rows)
+    wide = randn(2 * M, H + 2 * KVH + 1, D, seed=33).to(DEV)
+    q, k, v = wide[1::2, 1:1 + H], wide[::2, H:H + KVH], wide[1::2, -KVH:]
+    s, p, r = cuda(seq, pos, rope)
+    real = [i for i, x in enumerate(rows) if x in ((3, 5), (0, 130), (2, 700), (1, 64))]
+    for splits in (1, 2):
+        pool = cache.pool.clone()
+        idx = torch.tensor(real, device=DEV)
+        want, after = append_then_attend(cache, q[idx], k[idx], v[idx], torch.arange(4, dtype=I32, device=DEV), p[idx],
+                                         t[s[idx].long()].contiguous(), 701, splits, r, "interleaved", None, None)
+        out = torch.full((M, H + 1, D), 7.0, dtype=BF, device=DEV)
+        assert cache.step(q, k, v, s, p, t, max_kv=701, rope=r, eps=1e-5, splits=splits, out=out[:, :H]).data_ptr() == out.data_ptr()
+        assert torch.equal(out[idx][:, :H], want) and torch.equal(cache.pool, after)
+        rest = [i for i in range(M) if i not in real]
+        assert out[rest].eq(7.0).all() and out[:, H].eq(7.0).all()
+        cache.pool.copy_(pool)
+
+
+def test_a_step_with_nonfinite_inputs_and_a_negative_scale():
+    D, H, KVH = 64, 4, 2
+    at = [40, 70, 100, 0]
+    cache, t, qkv, rope, wq, wk, _, _ = setup_step(D, H, KVH, at, 0, False, seed=41)
+    qkv[0, 1, 3] = -math.inf                                       # a query
+    qkv[1, H + 1, 9] = math.nan                                    # a key
+    qkv[2, H + KVH, 40] = math.inf                                 # a value
+    d, s, p = cuda(qkv, torch.arange(4, dtype=I32), torch.tensor(at, dtype=I32))
+    q, k, v = d.split([H, KVH, KVH], dim=1)
+    want, pool = append_then_attend(cache, q, k, v, s, p, t, 101, 1, None, "interleaved", None, None, scale=-0.2)
+    got = cache.step(q, k, v, s, p, t, max_kv=101, scale=-0.2, splits=1)
+    assert same(got, want) and torch.equal(cache.pool, pool)
+    nan = torch.zeros(4, H, D, dtype=torch.bool)
+    nan[0, 1] = nan[1, 2:] = True
+    nan[2, :2, 32:] = True
+    assert torch.equal(got.isnan().cpu(), nan)
+
+
+def test_steps_in_a_captured_graph():
+    """A graph of a step whose inputs and positions change from replay to replay, with eager calls on the cache between them."""
+    D, H, KVH = 128, 8, 2
+    cache, t, qkv, rope, wq, wk, k0, v0 = setup_step(D, H, KVH, [800, 126], 128, True, seed=51)
+    wide = torch.full((2, t.shape[1] + 1), -1, dtype=I32)
+    wide[:, :t.shape[1]] = t.cpu()
+    wide[1, 2] = wide[0, -1] = -1
+    n_free = cache.n_pages                                         # two pages more: the second sequence grows into another
+    bigger = make_cache(n_free + 1, KVH, D, fill=0xFF)
+    bigger.pool[:n_free] = cache.pool
+    cache = bigger
+    wide[1, 2] = n_free
+    t, r, dq, dk = cuda(wide, rope, wq, wk)
+    s, pos = cuda(torch.arange(2, dtype=I32), torch.tensor([800, 126], dtype=I32))
+    d = torch.zeros(2, H + 2 * KVH, D, dtype=BF, device=DEV)
+    q, k, v = d.split([H, KVH, KVH], dim=1)
+    r = torch.cat([r, r[:10]])
+    for _ in range(2):                                             # (position 800 is written again by the first replay)
+        cache.step(q, k, v, s, pos, t, max_kv=2000, rope=r, q_norm=dq, k_norm=dk, eps=1e-5)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = cache.step(q, k, v, s, pos, t, max_kv=2000, rope=r, q_norm=dq, k_norm=dk, eps=1e-5)
+    for rep in range(5):
+        d.copy_(randn(2, H + 2 * KVH, D, seed=60 + rep))
+        pos.copy_(torch.tensor([800 + rep, 126 + rep], dtype=I32))
+        want, pool = append_then_attend(cache, q, k, v, s, pos, t, 2000, 0, r, "interleaved", dq, dk)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(cache.pool, pool)
+        cache.read(s, pos, t)
+
+
 def test_another_stream_and_captured_graphs_with_new_lengths():
     """Two graphs over one cache, replayed in turn with eager calls between them; lengths, rows and inputs live on the
     device and change from replay to replay."""
@@ -550,6 +682,7 @@ def test_empty_calls():
     s = torch.zeros(2, dtype=I32, device=DEV)
     out = cache.attend(torch.empty(0, 4, 64, dtype=BF, device=DEV), s, s[:1], t, max_q=0, max_kv=0)
     assert out.shape == (0, 4, 64)
+    assert cache.step(torch.empty(0, 4, 64, dtype=BF, device=DEV), z, z, e, e, t, max_kv=0).shape == (0, 4, 64)
     # no sequences at all: every row is one behind the last
     none, q = torch.empty(0, 2, dtype=I32, device=DEV), torch.ones(3, 4, 64, dtype=BF, device=DEV)
     assert cache.append(z, z, e, e, none) is None
