@@ -160,7 +160,7 @@ __device__ inline void kv4_store(uint8_t* blk, int tok, int sub, uint32_t codes,
 // products of the rotation are exact in fp32, one rounding of their sum, then bf16), so the stored codes do not depend on
 // how the lanes are arranged or on fused products.
 // Bound by memory for prompts: 16 384 tokens of 32 + 8 + 8 heads x 128 dims (12 288 bytes read, 8 192 of q and 1 088 of codes
-// written per token) take 67 to 74 us, 4.8 to 5.3 TB/s where a copy reaches 5.2.  One head per wave instead of eight: 108 us.
+// written per token) take 67 to 74 us, 4.8 to 5.3 TB/s where a copy reaches 5.2.  One head per wave instead of eight: 104 us.
 // Few tokens are bound by the launch (8 tokens: 2.2 to 3.4 us) and better off with every head in a wave of its own.
 template <int D, bool HALF, int HC>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
@@ -266,6 +266,8 @@ int launch_kv4_append(const Kv4AppendArgs& a, hipStream_t s) {
     FMI_REQUIRE(a.q_out != a.q || (a.q_out_stride == a.q_stride && !(a.rope && a.half)),
                 "kv4 append: q_out over q needs the same row stride and no half-split rotation");
   }
+  // one head per wave / eight, in us by the call's values: 32 + 16 heads x 128 dims 2^21.6 5.5 / 8.6, 2^22.6 9.4 / 10.6, 2^23.6 14.7 /
+  // 12.9, 2^26.6 104 / 73; 14 + 4 heads x 64 dims 2^22.2 8.0 / 9.7, 2^23.2 12.1 / 12.6, 2^24.2 19.3 / 18.8
   const bool half = a.rope && a.half, many = (int64_t)a.rows * (a.H + 2 * a.c.KVH) * D > (int64_t)1 << 23;
   const int hc = many ? 8 : 1;
   const dim3 grid = kv4_row_grid((a.H + hc - 1) / hc + 2 * ((a.c.KVH + hc - 1) / hc), a.rows, 4 * (64 / (D / 8)));
@@ -330,6 +332,8 @@ int launch_kv4_read(const Kv4ReadArgs& a, hipStream_t s) {
   FMI_REQUIRE(!a.row_seq == !a.row_pos, "kv4 read: null row indices");
   FMI_CHECK(kv4_check_rows("k", a.k, (int64_t)a.c.KVH * D, a.c.KVH, D));
   FMI_CHECK(kv4_check_rows("v", a.v, (int64_t)a.c.KVH * D, a.c.KVH, D));
+  // one block per wave / eight, in us by the values of K: 8 heads x 128 dims 2^19 3.4 / 3.6, 2^21 4.8 / 4.6, 2^22 7.1 / 6.4, 2^24 19.3 /
+  // 16.3; 2 heads x 64 dims 2^17 3.1 / 3.3, 2^20 4.0 / 3.8, 2^21 4.9 / 4.6
   const bool many = (int64_t)a.rows * a.c.KVH * D > (int64_t)1 << 21;
   const dim3 grid = kv4_row_grid((2 * a.c.KVH + (many ? 7 : 0)) / (many ? 8 : 1), a.rows, 4 * (64 / (D / 8)));
 #define FMI_KV4_READ(D_)                                                                              \
@@ -1032,7 +1036,8 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
 // and head, the ranges dealt over the groups of D / 4 lanes and their sums joined in group order.  grid (rows and heads of
 // the longest sequence, 4 / WPR to a work-group; n_seqs).  A group's first ranges are requested before the weights are
 // known: the two loads of a range wait for each other no more than once.  2.4 to 3.4 us for 8 rows x 32 heads x 4 ranges, 3.8
-// to 4.6 for 1 x 32 x 32: a launch and its latency.
+// to 4.6 for 1 x 32 x 32: a launch and its latency.  Attention and merge over 1 x 40k keys, one wave / four: 16 ranges 23.1 / 23.3
+// us, 24 20.9 / 19.7, 32 19.8 / 17.7, 64 25.3 / 19.3; 8 x 8k in 16 24.3 / 24.4, in 32 34.4 / 32.3.
 template <int D, int WPR>
 __global__ __launch_bounds__(256) void kv4_attn_merge_kernel(Kv4AttnArgs a) {
   constexpr int LN = D / 4, NG = 64 * WPR / LN, PRE = WPR == 1 ? 16 / NG : 4;

@@ -285,7 +285,7 @@ int64_t fmi_kv4_page_bytes(int n_kv_head, int head_dim);
 
 /* Rows of new tokens.  q / k / v: bf16, [heads][head_dim] contiguous within a row, rows `stride` elements apart (slices
  * of a fused q|k|v projection do); 16-byte aligned.  In order, all optional: head RMSNorm of q and k (q_norm_dev /
- * k_norm_dev, bf16 [head_dim], torch.nn.RMSNorm as llama.py:862-864), rotation of their first rope_dim dims (a multiple
+ * k_norm_dev, bf16 [head_dim], as llama.py:862-864), rotation of their first rope_dim dims (a multiple
  * of 16; rope_dev = bf16 [rope_len][rope_dim / 2][2] cos, sin by position; pairs (2 i, 2 i + 1) as llama.py:1026-1038,
  * or (i, i + rope_dim / 2) when rope_half); then k and v are stored and q goes to q_out_dev.
  * Row r belongs to position row_pos_dev[r] of sequence row_seq_dev[r]; a row whose sequence is outside [0, n_seqs), or
@@ -311,7 +311,7 @@ int fmi_op_kv4_append(const fmi_kv4_cache* cache, const fmi_kv4_rows* rows, void
 int fmi_op_kv4_read(const fmi_kv4_cache* cache, const int32_t* row_seq_dev, const int32_t* row_pos_dev, int rows,
                     void* k_out_dev, void* v_out_dev, void* stream);
 
-/* Causal attention over the cache (F.scaled_dot_product_attention, llama.py:928-934): sequence s has the query rows
+/* Causal attention over the cache (llama.py:928-934): sequence s has the query rows
  * q_start_dev[s] .. q_start_dev[s + 1] - 1 (int32 [n_seqs + 1], ascending) at its last positions, row i of n at position
  * kv_len_dev[s] - n + i, and sees the cached keys up to its own position; kv head = head / (n_head / n_kv_head).  fp32
  * scores, softmax and sums, one rounding to bf16.  A row that sees no key gives 0, one whose q holds an infinity or a NaN

@@ -177,3 +177,34 @@ def test_setup_refusals():
         other.read_kv4(0, 0, 0)
     assert other.lib.fmi_dualar_set_kv_bits(other._h, 4) == -3
     assert other.lib.fmi_dualar_set_kv_bits(other._h, 7) == -1
+
+
+def test_cli_and_worker_queue_options(tmp_path, monkeypatch):
+    """--kv-bits 4 and launch_thread_safe_queue(kv_bits=4) set the model's cache up in 4 bits; without them it is bf16."""
+    import numpy as np
+    from click.testing import CliRunner
+
+    from fish_speech_amd import text2semantic as T
+    from tests.test_cli_gpu import _s2_checkpoint
+
+    _s2_checkpoint(tmp_path, monkeypatch)
+    models = []
+    load = T.init_model
+
+    def init_model(*a, **k):
+        models.append(load(*a, **k))
+        return models[-1]
+
+    monkeypatch.setattr(T, "init_model", init_model)
+    args = ["--text", "<|speaker:0|>Hello there.", "--checkpoint-path", str(tmp_path), "--device", DEV, "--max-new-tokens", "9",
+            "--seed", "3", "--output-dir"]
+    for name, extra, bits in (("a", ["--kv-bits", "4"], 4), ("b", [], 16)):
+        r = CliRunner().invoke(T._cli(), args + [str(tmp_path / name)] + extra)
+        assert r.exit_code == 0, r.output + repr(r.exception)
+        codes = np.load(tmp_path / name / "codes_0.npy")
+        assert codes.shape[0] == 10 and 1 <= codes.shape[1] <= 8 and codes.min() >= 0 and codes.max() < 4096
+        assert models[-1][0].kv_bits == bits
+    assert CliRunner().invoke(T._cli(), args + [str(tmp_path / "c"), "--kv-bits", "8"]).exit_code != 0
+    queue = T.launch_thread_safe_queue(str(tmp_path), DEV, kv_bits=4)
+    queue.put(None)
+    assert models[-1][0].kv_bits == 4
