@@ -751,7 +751,11 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
 // page's codes in flight during a page's arithmetic.  Per page and wave:
 //   scores   S^T = K Q^T, v_mfma_f32_32x32x16_bf16, Q in registers for the whole kernel;
 //   softmax  as above; the probabilities are rounded to fp16 (11 bits: with bf16's 8 a second product with the remainder
-//            would be needed, half as much matrix work again) and stay in registers;
+//            would be needed, half as much matrix work again) and stay in registers.  fp16 has few powers of two, so all of
+//            them are used: probabilities are formed times 2^10, the reference m moves at 2^5, the largest is 2^15.  11 bits
+//            then hold down to 2^-24 of the reference's weight, and only what is under 2^-35 of it rounds to 0 (unlifted: 2^-14
+//            and 2^-25, which is where the keys beside an attention sink lie).  Moving m at 2^3 costs 2 % more (rescales),
+//            at 2^8 nothing less;
 //   output   O^T += V^T P, v_mfma_f32_32x32x16_f16, V^T by ds_read_b64_tr_b16.
 // V is kept in fp16 relative to 2^E, E = the largest block power among the pages so far (a page's 64 x D / 32 scale bytes are
 // one dword load and a maximum per wave): values are exact down to 2^-23 of the largest block's power, and what falls below
@@ -786,6 +790,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   constexpr int KROW = D * 2 + 16, VROW = D * 2 + (D > 32 ? 64 : 0);
   constexpr int PIECES = 2 * KV_PAGE * NB;                  // 16-byte pieces (32 codes) of K and V of a page
   constexpr int PPT = (PIECES + NT - 1) / NT;
+  constexpr float DEFER = 5.f, LIFT = 10.f;                 // powers of two: see "softmax" above
   __shared__ __attribute__((aligned(16))) unsigned char s_k[2][KV_PAGE * KROW];
   __shared__ __attribute__((aligned(16))) unsigned char s_v[2][KV_PAGE * VROW];
   __shared__ int s_nan[NB];
@@ -950,14 +955,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
 #pragma unroll
         for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sacc[kt][i]);
       mx = max_swap32(mx) * sl;
-      // the reference m moves only when a score exceeds it by 2^8: weights up to 256 are as exact in fp16 as weights up to 1,
-      // and O is seldom rescaled.  (mx is NaN for minus infinity times a scale of 0: no key seen, m stays.)
-      const float mn = mx > m + 8.f ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn);
+      // the reference m moves only when a score exceeds it by 2^5: O is seldom rescaled.  (mx is NaN for minus infinity times
+      // a scale of 0: no key seen, m stays.)
+      const float mn = mx > m + DEFER ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn), lift = LIFT - mn;
       float ps = 0.f;
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) sacc[kt][i] = __builtin_amdgcn_exp2f(fmaf(sacc[kt][i], sl, -mn));
+        for (int i = 0; i < 16; ++i) sacc[kt][i] = __builtin_amdgcn_exp2f(fmaf(sacc[kt][i], sl, lift));
       if (part && sl == 0.f) {      // (0 times minus infinity)
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -1010,7 +1015,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   if (wcol + c >= cols) return;
   // lane (c, h): dims dt * 32 + 8 (i / 4) + 4 h + i % 4 of column c; O is in units of 2^(E - 127)
   const int64_t idx = (int64_t)qrow * a.H + head;
-  const float inv = nz > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f;
+  const float inv = nz > 1 ? 0x1p-15f : l != 0.f ? 1.f / l : 0.f;    // partial states without the 2^(DEFER + LIFT)
 #pragma unroll
   for (int dt = 0; dt < NB; ++dt) {
     const bool bad = s_nan[dt] < vis;
@@ -1028,7 +1033,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   }
   if (nz > 1 && h == 0) {
     kv4_part_ml(a, z, idx)[0] = m;
-    kv4_part_ml(a, z, idx)[1] = l;
+    kv4_part_ml(a, z, idx)[1] = l * 0x1p-15f;
   }
 }
 
