@@ -424,7 +424,8 @@ __device__ inline float sum_swap16(float v) {
   return __uint_as_float(r[0]) + __uint_as_float(r[1]);
 }
 
-// 8 values of q.  Negated for a negative scale: the largest product is then the largest score.  With an infinity among them the
+// 8 values of q.  Negated for a negative scale: the largest product is then the largest score; 0 for a scale of 0, whose
+// products are left as they are (a hidden key's minus infinity times 0 would be NaN).  With an infinity among them the
 // scores are infinite or NaN and the row's softmax NaN; as NaNs from the start they cannot all be minus infinity, which would
 // pass for a row without keys.
 __device__ inline void kv4_prepare_q(u32x4& t, float scale) {
@@ -432,8 +433,12 @@ __device__ inline void kv4_prepare_q(u32x4& t, float scale) {
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) top = max(top, max(t[i] & 0x7fffu, (t[i] >> 16) & 0x7fffu));
+  if (scale == 0.f) t = (u32x4){0, 0, 0, 0};
   if (top >= 0x7f80u) t = (u32x4){0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
 }
+
+// scores in units of log2
+__device__ inline float kv4_log2_scale(float scale) { return scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f; }
 
 // ---- few query columns: tiles of 16, the kernel of single tokens.  NW waves; wave w takes the 32-key blocks w, w + NW, ...
 // of the range.  Per block:
@@ -579,7 +584,7 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
   int nan_key[NB];                               // first key whose V block is NaN, per 32-dim block
 #pragma unroll
   for (int i = 0; i < NB; ++i) nan_key[i] = INT32_MAX;
-  const float sl = fabsf(a.scale) * 1.4426950408889634f;   // scores in units of log2
+  const float sl = kv4_log2_scale(a.scale);
   unsigned char* sv = s_v[wave];
   const unsigned char* vr = sv + (g * 4 + (c >> 2)) * VROW + (c & 3) * 8;
 
@@ -656,16 +661,10 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
 #pragma unroll
       for (int i = 0; i < 8; ++i) mx = fmaxf(mx, t[i]);
       mx = max_swap32(max_swap16(mx)) * sl;
-      // the reference m moves only when a score exceeds it by 2^8: O is seldom rescaled, weights up to 256 lose nothing.  (mx is
-      // NaN for minus infinity times a scale of 0: no key seen, m stays.)
+      // the reference m moves only when a score exceeds it by 2^8: O is seldom rescaled, weights up to 256 lose nothing
       const float mn = mx > m + 8.f ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn);
 #pragma unroll
       for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f(fmaf(t[i], sl, -mn));
-      if (part && sl == 0.f) {      // (0 times minus infinity)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (!((i >> 2) * 16 + (i & 3) < lim)) t[i] = 0.f;
-      }
       l = l * corr + (((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7])));
       m = mn;
       u32x4 ph, pl;
@@ -757,10 +756,14 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
 //            and 2^-25, which is where the keys beside an attention sink lie).  Moving m at 2^3 costs 2 % more (rescales),
 //            at 2^8 nothing less;
 //   output   O^T += V^T P, v_mfma_f32_32x32x16_f16, V^T by ds_read_b64_tr_b16.
-// V is kept in fp16 relative to 2^E, E = the largest block power among the pages so far (a page's 64 x D / 32 scale bytes are
-// one dword load and a maximum per wave): values are exact down to 2^-23 of the largest block's power, and what falls below
-// is under 2^-24 of the largest value, the size of the rounding of the fp32 sums.  When E grows, O is scaled down like
-// with a growing maximum.
+// V is held in fp16 relative to 2^E, E = the largest block power of the range's first key, which every row sees that sees
+// any key of it.  fp16 is sound only while powers are alike: while every block's is within 2^-4 .. 2^5 of 2^E, V is exact and
+// the weights that round to 0 lose less than 2^-23 of the weights' sum of block powers per key (n keys under 2^-35, 7 * 2^(4 + 5)).
+// From the first key on that has another power (`first_out`; an all-zero block has the smallest there is), the rows that see
+// it go on in bf16, whose powers are fp32's: V exact, the weights as high and low part (16 bits), a second product.  The page
+// of that key is taken twice, for the rows before it in fp16 and for those from it on in bf16; what a row gives depends on no
+// key behind it, on no other row and not on the tile that it is in.  All in bf16 from the start: 18 to 22 % more time on
+// prompts of 2k tokens (8 over 4k keys 1.42 -> 1.73 ms), 7 % on 200.
 // Bound by issue: per page and wave 32 matrix instructions (34 % of the time) and 260 others (43 %), two waves per SIMD to
 // overlap them.  8 prompts of 2k tokens over 4k keys run at 960 TFLOP/s, two ragged ones at 850 (222 us; the last
 // work-groups run alone), 8 ragged prompts of up to 200 tokens in 14.5 us, mostly the latency of their 1 to 4 pages.
@@ -790,7 +793,8 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   constexpr int KROW = D * 2 + 16, VROW = D * 2 + (D > 32 ? 64 : 0);
   constexpr int PIECES = 2 * KV_PAGE * NB;                  // 16-byte pieces (32 codes) of K and V of a page
   constexpr int PPT = (PIECES + NT - 1) / NT;
-  constexpr float DEFER = 5.f, LIFT = 10.f;                 // powers of two: see "softmax" above
+  constexpr float DEFER = 5.f, LIFT = 10.f, UNLIFT = 0x1p-15f;   // powers of two: see "softmax" above
+  constexpr uint32_t BELOW = 4, ABOVE = 5;                  // V's powers around E
   __shared__ __attribute__((aligned(16))) unsigned char s_k[2][KV_PAGE * KROW];
   __shared__ __attribute__((aligned(16))) unsigned char s_v[2][KV_PAGE * VROW];
   __shared__ int s_nan[NB];
@@ -812,10 +816,12 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   const int wcol = col0 + 32 * wave;                        // this wave's first column
   const int col = min(wcol + c, cols - 1);
   const int qrow = sp.row0 + col / G, head = kvh * G + col % G;
-  const int vis = min(sp.pos0 + col / G + 1, sp.cached);       // keys [0, vis) are this column's
-  // keys that all / any of the wave's columns see (a wave behind the last column sees none)
-  const int all_see = min(sp.pos0 + min(wcol, cols - 1) / G + 1, sp.cached);
-  const int any_see = wcol < cols ? min(sp.pos0 + min(wcol + 31, cols - 1) / G + 1, sp.cached) : 0;
+  int vis = min(sp.pos0 + col / G + 1, sp.cached);             // keys [0, vis) are this column's (of the phase, below)
+  const int seen = vis;
+  // keys that all / any of the wave's columns see (a wave behind the last column sees none), and of the tile's
+  int all_see = min(sp.pos0 + min(wcol, cols - 1) / G + 1, sp.cached);
+  int any_see = wcol < cols ? min(sp.pos0 + min(wcol + 31, cols - 1) / G + 1, sp.cached) : 0;
+  const int tile_all = min(sp.pos0 + col0 / G + 1, sp.cached), tile_any = min(sp.pos0 + min(col0 + TC - 1, cols - 1) / G + 1, sp.cached);
   const int32_t* bt = a.c.block_table + (int64_t)sp.slot * a.c.max_pages;
 
   if (tid < NB) s_nan[tid] = INT32_MAX;
@@ -835,8 +841,8 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
 #pragma unroll
     for (int i = 0; i < 16; ++i) o[dt][i] = 0.f;
   float m = -FLT_MAX, l = 0.f;
-  int E = KV4_MIN_SCALE;
-  const float sl = fabsf(a.scale) * 1.4426950408889634f;   // scores in units of log2
+  int E = -1, first_out = INT32_MAX;                        // E: none yet
+  const float sl = kv4_log2_scale(a.scale);
 
   u32x4 code[PPT];
   uint32_t scale[PPT], vtok = 0;                            // vtok: the V scales of token `lane`
@@ -864,166 +870,207 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   int pg = p_lo, page = pg < p_hi ? bt[pg] : -1, next_page = pg + 1 < p_hi ? bt[pg + 1] : -1;
   if (pg < p_hi) fetch(page);
   __syncthreads();                                          // s_nan
-  for (int it = 0; pg < p_hi; ++pg, it ^= 1) {
-    const bool there = page >= 0 && page < a.c.n_pages;
-    const int tok_end = sp.cached - pg * KV_PAGE;           // tokens of the page at or past this are not the sequence's
-    float grow = 1.f;
-    if (there) {
-      // ---- E: the page's largest V block power
-      uint32_t top = 0;
+  int it = 0;
+  // the pages from pg on, whose codes are in flight.  FP16: up to that of first_out; EDGE: that page alone, in fp16; BF16: the rest
+  enum { FP16, EDGE, BF16 };
+  auto pages = [&](auto phase_) {
+    constexpr int PHASE = decltype(phase_)::value;
+    constexpr bool BF = PHASE == BF16;
+    for (; pg < p_hi; ++pg, it ^= 1) {
+      const bool there = page >= 0 && page < a.c.n_pages;
+      const int tok_end = sp.cached - pg * KV_PAGE;           // tokens of the page at or past this are not the sequence's
+      uint64_t hit = 0;
+      if (there) {
+        if constexpr (PHASE == FP16) {
+          if (E < 0) {
+            const int first = __builtin_amdgcn_readfirstlane((int)vtok);
+            E = 0;
 #pragma unroll
-      for (int i = 0; i < NB; ++i) {
-        const uint32_t b = (vtok >> (8 * i)) & 255u;
-        top = max(top, b == KV4_NAN_SCALE ? 0u : b);
-      }
-      const int pe = (int)wave_max_dpp_u(lane < tok_end ? top : 0u);
-      if (pe > E) {
-        grow = kv4_scale((uint32_t)max(127 + E - pe, 0));
-        E = pe;
-      }
-      // ---- stage
+            for (int i = 0; i < NB; ++i) {
+              const int b = (first >> (8 * i)) & 255;
+              E = max(E, b == KV4_NAN_SCALE ? 0 : b);
+            }
+          }
+          const uint32_t low = E - BELOW;
+          bool out = false;
 #pragma unroll
-      for (int i = 0; i < PPT; ++i) {
-        const int pc = tid + i * NT, isv = pc >= PIECES / 2, j = pc % (PIECES / 2), key = j / NB, part = j % NB;
-        if (PIECES % NT == 0 || pc < PIECES) {
-          if (!isv) {
-            const float ks = kv4_scale(scale[i]);
+          for (int i = 0; i < NB; ++i) out |= ((vtok >> (8 * i)) & 255u) - low > BELOW + ABOVE;
+          hit = __builtin_amdgcn_ballot_w64(out && lane < tok_end);
+        }
+        // ---- stage
 #pragma unroll
-            for (int w = 0; w < 4; ++w)
-              *reinterpret_cast<u32x4*>(&s_k[it][key * KROW + part * 64 + w * 16]) = kv4_unpack8(code[i][w], ks);
-          } else {
-            const bool use = key < tok_end, bad = use && scale[i] == KV4_NAN_SCALE;
-            if (bad) atomicMin(&s_nan[part], pg * KV_PAGE + key);
-            // (2^-31 and below round every value to 0; a masked block must not pass its scale on: 255 gives NaN even for 0)
-            const float vs = kv4_scale(use && !bad ? (uint32_t)max((int)scale[i] - E + 127, 96) : 127u);
-            u32x4 cw = use && !bad ? code[i] : (u32x4){0, 0, 0, 0};
-            const int turn = NB == 4 ? key & 3 : NB == 2 ? (key & 1) | ((key >> 1) & 2) : (key >> 2) & 3;
-            if (turn & 1) cw = (u32x4){cw[1], cw[2], cw[3], cw[0]};
-            if (turn & 2) cw = (u32x4){cw[2], cw[3], cw[0], cw[1]};
-            unsigned char* vw = &s_v[it][key * VROW + part * 64];
+        for (int i = 0; i < PPT; ++i) {
+          const int pc = tid + i * NT, isv = pc >= PIECES / 2, j = pc % (PIECES / 2), key = j / NB, part = j % NB;
+          if (PIECES % NT == 0 || pc < PIECES) {
+            if (!isv) {
+              const float ks = kv4_scale(scale[i]);
 #pragma unroll
-            for (int w = 0; w < 4; ++w) *reinterpret_cast<u32x4*>(vw + ((w + turn) & 3) * 16) = kv4_unpack8_f16(cw[w], vs);
+              for (int w = 0; w < 4; ++w)
+                *reinterpret_cast<u32x4*>(&s_k[it][key * KROW + part * 64 + w * 16]) = kv4_unpack8(code[i][w], ks);
+            } else {
+              const bool use = key < tok_end, bad = use && scale[i] == KV4_NAN_SCALE;
+              if (bad) atomicMin(&s_nan[part], pg * KV_PAGE + key);
+              // (a masked block must not pass its scale on: 255 gives NaN even for 0; V that no column of the phase sees stays finite)
+              const float vs = kv4_scale(!use || bad ? 127u : BF ? scale[i] : (uint32_t)min(max((int)scale[i] - E + 127, 96), 140));
+              u32x4 cw = use && !bad ? code[i] : (u32x4){0, 0, 0, 0};
+              const int turn = NB == 4 ? key & 3 : NB == 2 ? (key & 1) | ((key >> 1) & 2) : (key >> 2) & 3;
+              if (turn & 1) cw = (u32x4){cw[1], cw[2], cw[3], cw[0]};
+              if (turn & 2) cw = (u32x4){cw[2], cw[3], cw[0], cw[1]};
+              unsigned char* vw = &s_v[it][key * VROW + part * 64];
+#pragma unroll
+              for (int w = 0; w < 4; ++w)
+                *reinterpret_cast<u32x4*>(vw + ((w + turn) & 3) * 16) = BF ? kv4_unpack8(cw[w], vs) : kv4_unpack8_f16(cw[w], vs);
+            }
           }
         }
       }
-    }
-    __syncthreads();      // the page is staged; and every wave is done with the page before the previous one (same buffer)
-    if (pg + 1 < p_hi) fetch(next_page);
-    if (there && pg * KV_PAGE < any_see) {
-      // V^T fragments of 16 keys: lanes 4 r .. 4 r + 3 of a 16-lane group name row (key) r; lane i of the group gets dim i of
-      // the 4 rows.  The first are requested before the scores, the others a product ahead.
-      const unsigned char* vr = &s_v[it][(4 * h + ((lane & 15) >> 2)) * VROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8];
-      auto read_v = [&](int st, f16x8_t* f) {
+      if (__builtin_expect(hit != 0, 0)) {       // (asked here, the staging does not wait for it; what is staged is staged again)
+        first_out = pg * KV_PAGE + (int)__builtin_ctzll(hit);
+        if (first_out < tile_any) return;
+      }
+      __syncthreads();      // the page is staged; and every wave is done with the page before the previous one (same buffer)
+      if (PHASE != EDGE && pg + 1 < p_hi) fetch(next_page);
+      if (there && pg * KV_PAGE < any_see) {
+        // V^T fragments of 16 keys: lanes 4 r .. 4 r + 3 of a 16-lane group name row (key) r; lane i of the group gets dim i of
+        // the 4 rows.  The first are requested before the scores, the others a product ahead.
+        const unsigned char* vr = &s_v[it][(4 * h + ((lane & 15) >> 2)) * VROW + ((lane >> 4) & 1) * 32 + (lane & 3) * 8];
+        auto read_v = [&](int st, bf16x8* f) {
 #pragma unroll
-        for (int dt = 0; dt < NB; ++dt) {
-          const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + st * 16 * VROW + dt * 64));
-          const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + (st * 16 + 8) * VROW + dt * 64));
-          const bf16x8 t = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-          f[dt] = __builtin_bit_cast(f16x8_t, t);
-        }
-      };
-      f16x8_t vf[NB];
-      // ---- scores
-      f32x16 sacc[2];
-      bf16x8 kf[2][D / 16];
+          for (int dt = 0; dt < NB; ++dt) {
+            const s16x4_t v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + st * 16 * VROW + dt * 64));
+            const s16x4_t v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_t*)(vr + (st * 16 + 8) * VROW + dt * 64));
+            f[dt] = (bf16x8){v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+          }
+        };
+        bf16x8 vf[NB];
+        // ---- scores
+        f32x16 sacc[2];
+        bf16x8 kf[2][D / 16];
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk)
+            kf[kt][kk] = *reinterpret_cast<const bf16x8*>(&s_k[it][(kt * 32 + c) * KROW + h * 16 + kk * 32]);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sacc[0][i] = sacc[1][i] = 0.f;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk)
-          kf[kt][kk] = *reinterpret_cast<const bf16x8*>(&s_k[it][(kt * 32 + c) * KROW + h * 16 + kk * 32]);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) sacc[0][i] = sacc[1][i] = 0.f;
+          for (int kt = 0; kt < 2; ++kt) sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kt][kk], qf[kk], sacc[kt], 0, 0, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 2 * (D / 16), 0);   // the reads first
+        __builtin_amdgcn_sched_group_barrier(0x008, 2 * (D / 16), 0);
+        // ---- softmax: register i of tile kt is key kt * 32 + 8 (i / 4) + 4 h + i % 4 of column c
+        const bool part = pg * KV_PAGE + KV_PAGE > all_see;
+        const int lim = vis - pg * KV_PAGE - 4 * h;
+        float mx = -INFINITY;
+        if (part) {       // an unseen key's score is minus infinity whatever its K holds
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk)
+          for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt) sacc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[kt][kk], qf[kk], sacc[kt], 0, 0, 0);
-      __builtin_amdgcn_sched_group_barrier(0x100, 2 * (D / 16), 0);   // the reads first
-      __builtin_amdgcn_sched_group_barrier(0x008, 2 * (D / 16), 0);
-      // ---- softmax: register i of tile kt is key kt * 32 + 8 (i / 4) + 4 h + i % 4 of column c
-      const bool part = pg * KV_PAGE + KV_PAGE > all_see;
-      const int lim = vis - pg * KV_PAGE - 4 * h;
-      float mx = -INFINITY;
-      if (part) {       // an unseen key's score is minus infinity whatever its K holds
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!(kt * 32 + 8 * (i >> 2) + (i & 3) < lim)) sacc[kt][i] = -INFINITY;
-      }
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sacc[kt][i]);
-      mx = max_swap32(mx) * sl;
-      // the reference m moves only when a score exceeds it by 2^5: O is seldom rescaled.  (mx is NaN for minus infinity times
-      // a scale of 0: no key seen, m stays.)
-      const float mn = mx > m + DEFER ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn), lift = LIFT - mn;
-      float ps = 0.f;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) sacc[kt][i] = __builtin_amdgcn_exp2f(fmaf(sacc[kt][i], sl, lift));
-      if (part && sl == 0.f) {      // (0 times minus infinity)
+            for (int i = 0; i < 16; ++i)
+              if (!(kt * 32 + 8 * (i >> 2) + (i & 3) < lim)) sacc[kt][i] = -INFINITY;
+        }
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
-            if (!(kt * 32 + 8 * (i >> 2) + (i & 3) < lim)) sacc[kt][i] = 0.f;
+          for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sacc[kt][i]);
+        mx = max_swap32(mx) * sl;
+        // the reference m moves only when a score exceeds it by 2^5: O is seldom rescaled
+        const float mn = mx > m + DEFER ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn), lift = (BF ? -DEFER : LIFT) - mn;
+        float ps = 0.f;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) sacc[kt][i] = __builtin_amdgcn_exp2f(fmaf(sacc[kt][i], sl, lift));
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) ps += sacc[kt][i];
+        l = l * corr + ps;
+        m = mn;
+        read_v(0, vf);
+        if (__builtin_amdgcn_ballot_w64(corr != 1.f)) {
+#pragma unroll
+          for (int dt = 0; dt < NB; ++dt)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[dt][i] *= corr;
+        }
+        // ---- O^T += V^T P, 16 keys per product: slots (h, 0..3) = keys 4 h .., slots (h, 4..7) = keys 8 + 4 h ..
+        auto weights = [&](int st, int i) { return sacc[st >> 1][(st & 1) * 8 + i]; };
+        u32x4 pf[4], pl[4];
+#pragma unroll
+        for (int st = 0; st < 4; ++st)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float t0 = weights(st, 2 * i), t1 = weights(st, 2 * i + 1);
+            pf[st][i] = BF ? kv4_pk_bf16(t0, t1) : kv4_pk_f16(t0, t1);
+            if constexpr (BF) pl[st][i] = kv4_pk_bf16(t0 - bf_lo(pf[st][i]), t1 - bf_hi(pf[st][i]));
+          }
+#pragma unroll
+        for (int st = 0; st < 4; ++st) {
+          bf16x8 vn[NB];
+          if (st < 3) read_v(st + 1, vn);
+#pragma unroll
+          for (int dt = 0; dt < NB; ++dt) {
+            if constexpr (BF) {
+              o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[dt], __builtin_bit_cast(bf16x8, pf[st]), o[dt], 0, 0, 0);
+              o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[dt], __builtin_bit_cast(bf16x8, pl[st]), o[dt], 0, 0, 0);
+            } else {
+              o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, vf[dt]),
+                                                             __builtin_bit_cast(f16x8_t, pf[st]), o[dt], 0, 0, 0);
+            }
+          }
+#pragma unroll
+          for (int dt = 0; dt < NB; ++dt) vf[dt] = vn[dt];
+        }
       }
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) ps += sacc[kt][i];
-      l = l * corr + ps;
-      m = mn;
-      const float oc = corr * grow;
-      read_v(0, vf);
-      if (__builtin_amdgcn_ballot_w64(oc != 1.f)) {
-#pragma unroll
-        for (int dt = 0; dt < NB; ++dt)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[dt][i] *= oc;
+      if constexpr (PHASE == EDGE) {
+        it ^= 1;
+        return;
       }
-      // ---- O^T += V^T P, 16 keys per product: slots (h, 0..3) = keys 4 h .., slots (h, 4..7) = keys 8 + 4 h ..
-      u32x4 pf[4];
-#pragma unroll
-      for (int st = 0; st < 4; ++st)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) pf[st][i] = kv4_pk_f16(sacc[st >> 1][(st & 1) * 8 + 2 * i], sacc[st >> 1][(st & 1) * 8 + 2 * i + 1]);
-#pragma unroll
-      for (int st = 0; st < 4; ++st) {
-        f16x8_t vn[NB];
-        if (st < 3) read_v(st + 1, vn);
-#pragma unroll
-        for (int dt = 0; dt < NB; ++dt)
-          o[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[dt], __builtin_bit_cast(f16x8_t, pf[st]), o[dt], 0, 0, 0);
-#pragma unroll
-        for (int dt = 0; dt < NB; ++dt) vf[dt] = vn[dt];
-      }
-    } else if (grow != 1.f) {
-#pragma unroll
-      for (int dt = 0; dt < NB; ++dt)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[dt][i] *= grow;
+      page = next_page;
+      next_page = pg + 2 < p_hi ? bt[pg + 2] : -1;
     }
-    page = next_page;
-    next_page = pg + 2 < p_hi ? bt[pg + 2] : -1;
+  };
+  pages(std::integral_constant<int, FP16>{});
+  if (__builtin_expect(pg < p_hi && tile_all <= first_out, 0)) {
+    const int any = any_see;
+    vis = seen > first_out ? 0 : seen;
+    any_see = all_see > first_out ? 0 : any_see;
+    pages(std::integral_constant<int, EDGE>{});
+    any_see = any;
+  }
+  float unit = E >= 0 ? kv4_scale((uint32_t)max(E, KV4_MIN_SCALE)) * UNLIFT : 1.f;    // of O; l's is UNLIFT
+  if (__builtin_expect(pg < p_hi, 0)) {
+#pragma unroll
+    for (int dt = 0; dt < NB; ++dt)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[dt][i] *= unit;
+    l *= UNLIFT;
+    unit = 1.f;
+    vis = seen > first_out ? seen : 0;
+    all_see = all_see > first_out ? all_see : 0;
+    any_see = any_see > first_out ? any_see : 0;
+    fetch(page);
+    pages(std::integral_constant<int, BF16>{});
+  } else {
+    l *= UNLIFT;
   }
 
   l = sum_swap32(l);
   __syncthreads();        // s_nan is complete
   if (wcol + c >= cols) return;
-  // lane (c, h): dims dt * 32 + 8 (i / 4) + 4 h + i % 4 of column c; O is in units of 2^(E - 127)
+  // lane (c, h): dims dt * 32 + 8 (i / 4) + 4 h + i % 4 of column c
   const int64_t idx = (int64_t)qrow * a.H + head;
-  const float inv = nz > 1 ? 0x1p-15f : l != 0.f ? 1.f / l : 0.f;    // partial states without the 2^(DEFER + LIFT)
+  const float inv = nz > 1 ? 1.f : l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
   for (int dt = 0; dt < NB; ++dt) {
-    const bool bad = s_nan[dt] < vis;
+    const bool bad = s_nan[dt] < seen;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       f32x4 r;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = bad ? __uint_as_float(0x7fc00000u) : ldexpf(o[dt][q * 4 + j] * inv, E - 127);
+      for (int j = 0; j < 4; ++j) r[j] = bad ? __uint_as_float(0x7fc00000u) : o[dt][q * 4 + j] * inv * unit;
       const int d = dt * 32 + q * 8 + h * 4;
       if (nz == 1)
         *reinterpret_cast<uint2*>(a.out + qrow * a.out_stride + (int64_t)head * D + d) = make_uint2(kv4_pk_bf16(r[0], r[1]), kv4_pk_bf16(r[2], r[3]));
@@ -1033,7 +1080,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   }
   if (nz > 1 && h == 0) {
     kv4_part_ml(a, z, idx)[0] = m;
-    kv4_part_ml(a, z, idx)[1] = l * 0x1p-15f;
+    kv4_part_ml(a, z, idx)[1] = l;
   }
 }
 

@@ -319,7 +319,8 @@ int fmi_op_kv4_read(const fmi_kv4_cache* cache, const int32_t* row_seq_dev, cons
  * sequence are not computed).  splits: key ranges a query tile is divided into, 1 .. 256, or 0 for a choice made from
  * n_seqs, max_q and max_kv alone; with a fixed value (and max_q) a row's bits do not depend on the other sequences of the
  * call.  Up to 64 query columns (max_q times heads per kv head) the softmax weights enter the product with 16 significant
- * bits, above that with fp16's 11: in full down to 2^-24 of the row's largest weight, in steps of 2^-35 of it below. */
+ * bits, above that with fp16's 11: in full down to 2^-24 of the row's largest weight, in steps of 2^-35 of it below.  Rows
+ * that see a V block whose power is not within 2^-4 .. 2^5 of the first key's take 16 bits there too, at any weight. */
 typedef struct fmi_kv4_query {
   const void* q_dev;
   int64_t q_stride;

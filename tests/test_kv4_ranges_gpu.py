@@ -84,3 +84,117 @@ def test_keys_beside_an_attention_sink(D, H, KVH, rows, gap, splits):
     below = (s[..., :1] - s[..., 1:keys - rows]).median()
     assert gap - 1 <= below <= gap + 1                              # (of the stored keys)
     assert worst(got, ref, tol) <= 1
+
+
+# ------------------------------------------------------------------------------------------------ V of very different powers
+
+
+def spread_case(D, H, KVH, keys, power, seed):
+    """V normal times 2^power, a tensor that spreads over (keys, KVH, D)."""
+    q, k = randn(keys, H, D, seed=seed), randn(keys, KVH, D, seed=seed + 1)
+    v = (torch.randn(keys, KVH, D, generator=torch.Generator().manual_seed(seed + 2)).double() * 2.0 ** power.double()).to(BF)
+    return q, k, v
+
+
+@pytest.mark.parametrize("D, H, KVH", [(128, 8, 2), (64, 4, 2), (32, 3, 3)])
+@pytest.mark.parametrize("small", [-20, -30, -60, -90])
+@pytest.mark.parametrize("big_at", [1, 31, 40, 63, 64, 100, 195])
+def test_a_large_value_leaves_the_rows_before_it_alone(D, H, KVH, small, big_at):
+    keys = 200
+    power = torch.full((keys, 1, 1), small)
+    power[big_at] = 0
+    q, k, v = spread_case(D, H, KVH, keys, power, 3)
+    cache, t, ks, vs = stored_cache(k, v)
+    got = attend(cache, t, q, keys)
+    ref, tol = reference(q, ks, vs, 1 / math.sqrt(D), 2.0 ** -11)
+    assert worst(got, ref, tol) <= 1
+    # the few-row kernel, on the rows around the large value
+    lo, n = max(0, big_at - 3), 6
+    few = attend(cache, t, q[lo:lo + n], min(lo + n, keys))
+    ref, tol = reference(q[lo:lo + n], ks[:lo + n], vs[:lo + n], 1 / math.sqrt(D), 2.0 ** -16)
+    assert worst(few, ref, tol) <= 1
+
+
+def powers(kind, keys, KVH, D):
+    g = torch.Generator().manual_seed(11)
+    if kind == "dims":                # one 32-dim block after the other, 2^40 apart
+        return (torch.arange(D) // 32 * 40 - 60).expand(keys, KVH, D)
+    if kind == "falling":             # page after page, 2^35 down
+        return (40 - torch.arange(keys) // 64 * 35)[:, None, None]
+    if kind == "rising":
+        return (-90 + torch.arange(keys) // 64 * 35)[:, None, None]
+    if kind == "window":              # about the powers that the prompt kernel holds in fp16, and a step beyond
+        return torch.randint(-5, 7, (keys, KVH, D // 32), generator=g).repeat_interleave(32, -1)
+    return torch.randint(-95, 100, (keys, KVH, D // 32), generator=g).repeat_interleave(32, -1)    # "random"
+
+
+@pytest.mark.parametrize("D, H, KVH", [(128, 8, 2), (64, 4, 2), (32, 6, 2)])
+@pytest.mark.parametrize("kind", ["dims", "falling", "rising", "window", "random"])
+@pytest.mark.parametrize("rows, splits", [(300, 1), (60, 1), (3, 1), (60, 2), (3, 3)])
+def test_powers_spread_over_blocks_tokens_and_pages(D, H, KVH, kind, rows, splits):
+    keys = 300 if splits == 1 else 1000
+    q, k, v = spread_case(D, H, KVH, keys, powers(kind if splits == 1 or kind not in ("falling", "rising") else "random", keys, KVH, D), 5)
+    q = q[-rows:]
+    cache, t, ks, vs = stored_cache(k, v)
+    got = attend(cache, t, q, keys, splits)
+    ref, tol = reference(q, ks, vs, 1 / math.sqrt(D), weight_bits(rows, H // KVH))
+    assert worst(got, ref, tol) <= 1
+
+
+@pytest.mark.parametrize("D, H, KVH", [(128, 8, 2), (64, 4, 2), (32, 6, 2)])
+@pytest.mark.parametrize("rows", [60, 16, 1])
+@pytest.mark.parametrize("gap", [20.0, 26.0])
+def test_keys_far_below_a_sink_without_a_value(D, H, KVH, rows, gap):
+    """Weights about 2^-29 and 2^-37, all that there is where the sink's V is 0."""
+    keys = 1500
+    q, k, v = sink_case(D, H, KVH, rows, keys, gap, 21, torch.zeros(D))
+    cache, t, ks, vs = stored_cache(k, v)
+    for splits in (1, 2):
+        got = attend(cache, t, q, keys, splits)
+        ref, tol = reference(q, ks, vs, 1 / math.sqrt(D), weight_bits(rows, H // KVH))
+        assert worst(got, ref, tol) <= 1
+
+
+@pytest.mark.parametrize("D, H, KVH", [(128, 8, 2), (64, 6, 2), (32, 3, 1)])
+@pytest.mark.parametrize("odd", [None, 0, 1, 37, 64, 130, 191, 199])
+def test_a_prompts_rows_do_not_depend_on_later_tokens_or_on_how_it_is_cut(D, H, KVH, odd):
+    """Bit for bit, with one token (`odd`) whose V is 2^30 times the others', and with none; the last tokens replaced by
+    other ones; the prompt in two calls, cut at every kind of place (each call has more than 64 query columns)."""
+    keys = 260
+    power = torch.zeros(keys, 1, 1)
+    if odd is not None:
+        power[odd] = 30
+    q, k, v = spread_case(D, H, KVH, keys, power, 9)
+    cache, t, _, _ = stored_cache(k, v)
+    whole = attend(cache, t, q, keys)
+    for cut in (66, 128, 131, 190):
+        first, second = attend(cache, t, q[:cut], cut), attend(cache, t, q[cut:], keys)
+        assert torch.equal(first, whole[:cut]) and torch.equal(second, whole[cut:]), cut
+        v2 = v.clone()
+        v2[cut:] = (v2[cut:].float() * 2.0 ** torch.randint(-60, 60, (keys - cut, 1, 1), generator=torch.Generator().manual_seed(cut))).to(BF)
+        other, t2, _, _ = stored_cache(k, v2)
+        assert torch.equal(attend(other, t2, q, keys)[:cut], whole[:cut]), cut
+
+
+def test_nan_blocks_and_missing_pages_at_the_start_of_a_prompt():
+    """A first key whose V is NaN in one block, or in all; a first page that is not there."""
+    D, H, KVH, keys = 64, 4, 2, 200
+    q, k, v = spread_case(D, H, KVH, keys, torch.zeros(keys, 1, 1), 13)
+    for dims in (slice(0, 1), slice(0, 64, 32)):
+        bad = v.clone()
+        bad[0, 1, dims] = math.nan
+        cache, t, ks, vs = stored_cache(k, bad)
+        got = attend(cache, t, q, keys).cpu()
+        nan = torch.zeros(keys, H, D, dtype=torch.bool)
+        nan[:, 2:, :32] = True
+        if dims.step:
+            nan[:, 2:, 32:] = True
+        assert torch.equal(got.isnan(), nan)
+        ref, tol = reference(q, ks, vs.nan_to_num(0.0), 1 / math.sqrt(D), 2.0 ** -11)
+        assert bool(((got.double() - ref).abs() <= tol)[~nan].all())
+    cache, t, ks, vs = stored_cache(k, v)
+    t[0, 0] = -1
+    got = attend(cache, t, q, keys)
+    assert got[:64].eq(0).all()
+    ref, tol = reference(q[64:], ks[64:], vs[64:], 1 / math.sqrt(D), 2.0 ** -11)
+    assert worst(got[64:], ref, tol) <= 1
