@@ -469,6 +469,7 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
                                                  // group reads together lie in different banks
   constexpr int VL = D / 32, VP = 64 / VL;       // lanes per key and keys per pass of the V unpacking
   constexpr int VPASS = VP >= KB ? 1 : KB / VP;
+  constexpr float DEFER = 8.f;
   __shared__ __attribute__((aligned(16))) unsigned char s_v[NW][KB * VROW];
   __shared__ float s_m[NW][16], s_l[NW][16];
   __shared__ int s_nan[NW][NB];
@@ -661,10 +662,11 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
 #pragma unroll
       for (int i = 0; i < 8; ++i) mx = fmaxf(mx, t[i]);
       mx = max_swap32(max_swap16(mx)) * sl;
-      // the reference m moves only when a score exceeds it by 2^8: O is seldom rescaled, weights up to 256 lose nothing
-      const float mn = mx > m + 8.f ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn);
+      // the reference m moves only when a score exceeds it by 2^8: O is seldom rescaled.  Weights are relative to the most it
+      // can be exceeded by, so none is above 1 and O no larger than with the true maximum (V may be as large as 2^127).
+      const float mn = mx > m + DEFER ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn), top = mn + DEFER;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f(fmaf(t[i], sl, -mn));
+      for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f(fmaf(t[i], sl, -top));
       l = l * corr + (((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7])));
       m = mn;
       u32x4 ph, pl;

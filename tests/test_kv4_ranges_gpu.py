@@ -198,3 +198,20 @@ def test_nan_blocks_and_missing_pages_at_the_start_of_a_prompt():
     assert got[:64].eq(0).all()
     ref, tol = reference(q[64:], ks[64:], vs[64:], 1 / math.sqrt(D), 2.0 ** -11)
     assert worst(got[64:], ref, tol) <= 1
+
+
+@pytest.mark.parametrize("D, H, KVH", [(128, 8, 2), (64, 4, 2), (32, 3, 3)])
+@pytest.mark.parametrize("rows", [1, 16, 70])
+@pytest.mark.parametrize("power", [-99, 112, 116])
+def test_sums_of_large_and_small_values_stay_in_range(D, H, KVH, rows, power):
+    """Scores that rise to 2^7.5 of the first ones' weight (less than a running maximum may lag behind): no sum is larger
+    than with the true maximum, 1500 times 2^116 at most, and small values keep their bits."""
+    keys = 1500
+    q, k = torch.ones(rows, H, D, dtype=BF), torch.zeros(keys, KVH, D, dtype=BF)
+    k[256:] = 0.75
+    v = ((1 + randn(keys, KVH, D, seed=3).double() * 0.1) * 2.0 ** power).to(BF)
+    scale = 7.5 * math.log(2) / (0.75 * D)
+    cache, t, ks, vs = stored_cache(k, v)
+    ref, tol = reference(q, ks, vs, scale, weight_bits(rows, H // KVH))
+    for splits in (1, 3):
+        assert worst(attend(cache, t, q, keys, splits, scale=scale), ref, tol) <= 1, splits
