@@ -382,8 +382,8 @@ class MiDualAR:
         if self.max_seq_len >= max_seq_len and self.max_batch_size >= max_batch_size:
             return
         check(self.lib.fmi_dualar_set_kv_bits(self._h, int(kv_bits)))
-        self.kv_bits = kv_bits
         check(self.lib.fmi_dualar_setup_caches(self._h, int(max_batch_size), int(max_seq_len)))
+        self.kv_bits = kv_bits          # (a refused call chooses nothing)
         self.max_batch_size, self.max_seq_len = max_batch_size, max_seq_len
         self._cache_setup_done = True
 

@@ -252,3 +252,37 @@ BF = torch.bfloat16
 def test_python_argument_errors(cache, what, kw):
     with pytest.raises(ValueError):
         _call(cache, what, **kw)
+
+
+# ------------------------------------------------------------------------------------------------ the model's setup
+
+
+class _Handle:
+    """The library's part of MiDualAR.setup_caches: caches of at most 1024 positions."""
+
+    def __init__(self):
+        self.bits, self.calls = 16, []
+
+    def fmi_dualar_set_kv_bits(self, h, bits):
+        self.bits = bits
+        return 0
+
+    def fmi_dualar_setup_caches(self, h, max_batch, max_seq_len):
+        self.calls.append((self.bits, max_batch, max_seq_len))
+        return -1 if max_seq_len > 1024 else 0
+
+
+def test_a_refused_setup_does_not_choose_the_caches_type():
+    from fish_speech_amd.dual_ar import MiDualAR
+
+    m = MiDualAR.__new__(MiDualAR)
+    m.lib, m._h = _Handle(), None
+    m._cache_setup_done, m.max_batch_size, m.max_seq_len, m.kv_bits = False, -1, -1, 16
+    with pytest.raises(FishmiError):
+        m.setup_caches(1, 2048, kv_bits=4)
+    assert m.kv_bits == 16 and not m._cache_setup_done
+    m.setup_caches(1, 512)
+    assert m.kv_bits == 16 and m.lib.calls == [(4, 1, 2048), (16, 1, 512)]
+    m.setup_caches(1, 256, kv_bits=16)
+    with pytest.raises(FishmiError, match="already set up"):
+        m.setup_caches(1, 256, kv_bits=4)
