@@ -367,8 +367,9 @@ int block_slow_rest(fmi_dualar* h, const LayerW& w, bf16_t* x, int rows, hipStre
 
 // K/V append and attention over the 4-bit cache: ws.qkv -> ws.ao, one launch for a decode step.  The key ranges of a step are a
 // function of the row's own position (kv4_attn_ranges under a fixed KV4_SPLITS); prompts run in one range and always on the
-// wide tiles, also the few rows of a resumed one: an utterance's numbers do not depend on its batch-mates or on how its prompt
-// was cut.
+// wide tiles, also the few rows of a resumed one: the attention of an utterance does not depend on its batch-mates or on how
+// its prompt was cut.  (Its projections do: calls of up to 16 rows in all sum in another order than longer ones, and a last-bit
+// difference may move a stored 4-bit value by a step.)
 constexpr int KV4_SPLITS = 16;
 int attn_kv4(fmi_dualar* h, const LayerW& w, int layer, int rows, const int32_t* row_slot, const int32_t* row_pos, hipStream_t s) {
   const Dims& d = h->slow;
@@ -386,7 +387,7 @@ int attn_kv4(fmi_dualar* h, const LayerW& w, int layer, int rows, const int32_t*
   if (!row_pos) {
     p.slot_pos = h->st.pos; p.slot_done = h->st.done;
     a.part = h->kv4_part;
-    a.splits = (h->attn_mask & 2) ? KV4_SPLITS : 1;   // (bit 2 unset: no row is long enough to be split, the merge launch is saved)
+    a.splits = h->attn_mask ? KV4_SPLITS : 1;   // (0: no row is long enough to be split, the merge launch is saved)
     FMI_CHECK(launch_kv4_step(p, a, s));
     h->launches += a.splits > 1 ? 2 : 1;
     return FMI_OK;
@@ -478,9 +479,10 @@ int block_fast(fmi_dualar* h, const LayerW& w, int layer, bf16_t* x, int B, int 
 }
 
 // attn_mask of a frame or frames in which a row's position reaches `last`, the lowest being `first`: which decode attention
-// kernels the frames launch (bf16 cache) or whether rows are split over key ranges (4-bit cache)
+// kernels the frames launch (bf16 cache) or whether rows are split over key ranges (4-bit cache: 2 if one is, else 0, so that
+// rows of both kinds share the graph of the split ones)
 int attn_mask_of(const fmi_dualar* h, int first, int last) {
-  if (h->kv_bits == 4) return last + 1 > (KV4_SINGLE_PAGES - 1) * KV_PAGE ? 2 : 1;
+  if (h->kv_bits == 4) return last + 1 > (KV4_SINGLE_PAGES - 1) * KV_PAGE ? 2 : 0;
   if (h->attn_long_thr <= 0) return 1;
   return (first < h->attn_long_thr ? 1 : 0) | (last >= h->attn_long_thr ? 2 : 0);
 }

@@ -208,3 +208,25 @@ def test_cli_and_worker_queue_options(tmp_path, monkeypatch):
     queue = T.launch_thread_safe_queue(str(tmp_path), DEV, kv_bits=4)
     queue.put(None)
     assert models[-1][0].kv_bits == 4
+
+
+def test_short_and_long_rows_share_the_graph_of_the_long_ones():
+    """Two slots, both past the length from which rows are split, then a short one beside a long one: the second call replays
+    the first one's graph (the launch count is that of the frame built last: an eager one in between)."""
+    cfg = _cfg("mid", 1024)
+    state = O.make_synthetic_state(cfg, seed=8, head_gain=8.0)
+    model = _model(cfg, state, 3)
+    model.set_ignore_eos(True)
+    samp = model._sampling(0.7, 0.7, 1, 9, True)
+    prompts = [O.make_prompt(cfg, T, seed=T, n_semantic=3) for T in (800, 750, 40)]
+    model.prefill([0, 1, 2], prompts, [60] * 3, [samp] * 3)
+    model.decode([0, 1], 2)
+    split = model.last_decode_stats()[1]
+    model.set_graph(False)
+    model.decode([2], 1)
+    single = model.last_decode_stats()[1]
+    assert single < split                                          # no merge launches
+    model.set_graph(True)
+    model.decode([0, 2], 2)
+    assert model.last_decode_stats()[1] == single                  # no frame was built
+    model.synchronize()
