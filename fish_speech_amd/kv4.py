@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import functools
 import math
+import operator
 import struct
 from typing import Optional, Tuple
 
@@ -40,13 +41,35 @@ def page_bytes(n_kv_head: int, head_dim: int) -> int:
 @functools.lru_cache(maxsize=1024)
 def _attention_ws_bytes(n_kv_head: int, head_dim: int, n_head: int, n_seqs: int, rows: int, max_q: int, max_kv: int,
                         splits: int) -> int:
-    """fmi_kv4_attention_ws_bytes: a function of these sizes alone"""
+    """fmi_kv4_attention_ws_bytes: a function of these sizes alone (which are checked where they are new)"""
+    for name, v in (("max_q", max_q), ("max_kv", max_kv), ("splits", splits)):
+        if not -1 << 31 <= v < 1 << 31:
+            raise ValueError(f"{name} must be a number of 32 bits, not {v}")
     c = _CACHE.pack(0, 0, 1, n_kv_head, head_dim, n_seqs, 1)
     q = _QUERY.pack(0, 0, n_head, 0, 0, n_seqs, rows, max_q, max_kv, 1.0, splits)
     n = _lib.load().fmi_kv4_attention_ws_bytes(c, q)
     if n < 0:
         check(int(n))
     return int(n)
+
+
+def _whole(name: str, v) -> int:
+    """v, or what it stands for now (a one-element tensor), as an int"""
+    try:
+        return operator.index(v)
+    except TypeError:
+        raise ValueError(f"{name} must be a whole number, not {v!r}") from None
+
+
+def _real(name: str, v) -> float:
+    """v as a float that fits an fp32 field (inf and NaN pass: the library refuses them where they mean nothing)"""
+    try:
+        f = float(v)
+    except (TypeError, ValueError):
+        raise ValueError(f"{name} must be a number, not {v!r}") from None
+    if math.isfinite(f) and abs(f) > 3.4028234663852886e38:
+        raise ValueError(f"{name} {f} is out of the range of fp32")
+    return f
 
 
 class KV4Cache:
@@ -166,6 +189,8 @@ class KV4Cache:
             qn = self._weight("q_norm", q_norm)
         if k_norm is not None:
             kn = self._weight("k_norm", k_norm)
+        if type(eps) is not float:
+            eps = _real("eps", eps)
         return _ROWS.pack(qp, k.data_ptr(), v.data_ptr(), qs, ks, vs, op, os, heads, qn, kn, eps, rp, rl, rd,
                           rope_layout == "half", ps, pp, rows)
 
@@ -193,10 +218,15 @@ class KV4Cache:
             out, os = self._new(n, heads), heads * self.head_dim
         else:
             os = self._rows("out", out, n, heads)
-        if scale is None:
-            scale = 1.0 / math.sqrt(self.head_dim)
-        a = _QUERY.pack(q.data_ptr(), qs, heads, sp, lp, n_seqs, n, max_q, max_kv, scale, splits)
+        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else _real("scale", scale)
+        if type(max_q) is not int:
+            max_q = _whole("max_q", max_q)
+        if type(max_kv) is not int:
+            max_kv = _whole("max_kv", max_kv)
+        if type(splits) is not int:
+            splits = _whole("splits", splits)
         need = _attention_ws_bytes(self.n_kv_head, self.head_dim, heads, n_seqs, n, max_q, max_kv, splits)
+        a = _QUERY.pack(q.data_ptr(), qs, heads, sp, lp, n_seqs, n, max_q, max_kv, scale, splits)
         if need:           # from torch's allocator: ordered with the stream, private to a graph that is being captured
             ws = torch.empty(need, dtype=torch.uint8, device=self.device)
             self._call(self.lib.fmi_op_kv4_attention, c, a, out.data_ptr(), os, ws.data_ptr(), need)
@@ -219,8 +249,11 @@ class KV4Cache:
             out, os = self._new(rows, heads), heads * self.head_dim
         else:
             os = self._rows("out", out, rows, heads)
-        if scale is None:
-            scale = 1.0 / math.sqrt(self.head_dim)
+        scale = 1.0 / math.sqrt(self.head_dim) if scale is None else _real("scale", scale)
+        if type(max_kv) is not int:
+            max_kv = _whole("max_kv", max_kv)
+        if type(splits) is not int:
+            splits = _whole("splits", splits)
         need = _attention_ws_bytes(self.n_kv_head, self.head_dim, max(heads, 1), rows, rows, 1, max_kv, splits)
         ws = torch.empty(need, dtype=torch.uint8, device=self.device) if need else None    # (as in attend)
         self._call(self.lib.fmi_op_kv4_step, self._cache(block_table), a, scale, max_kv, splits, out.data_ptr(), os,

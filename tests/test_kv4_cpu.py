@@ -286,3 +286,31 @@ def test_a_refused_setup_does_not_choose_the_caches_type():
     m.setup_caches(1, 256, kv_bits=16)
     with pytest.raises(FishmiError, match="already set up"):
         m.setup_caches(1, 256, kv_bits=4)
+
+
+@pytest.mark.parametrize("what, kw", [
+    ("attend", dict(max_q=1 << 31)), ("attend", dict(max_kv=1 << 40)), ("attend", dict(max_q=2.0)), ("attend", dict(max_kv=None)),
+    ("attend", dict(max_q=torch.tensor(3.0))), ("attend", dict(splits=1 << 31)), ("attend", dict(splits="2")), ("attend", dict(scale="x")),
+    ("attend", dict(scale=1e50)), ("step", dict(max_kv=1 << 31)), ("step", dict(splits=2.5)), ("step", dict(scale=torch.ones(2))),
+    ("step", dict(scale=-1e39)), ("step", dict(eps="x")), ("append", dict(eps=None))], ids=str)
+def test_numbers_that_are_none_or_out_of_range(cache, what, kw, monkeypatch):
+    """A ValueError of the argument's name, not one of the packing's; outputs are not what is refused here."""
+    monkeypatch.setattr(cache, "_new", lambda rows, heads: torch.zeros(rows, heads, 64, dtype=BF), raising=False)
+    with pytest.raises(ValueError, match=next(iter(kw))):
+        _call(cache, what, **kw)
+
+
+def test_numbers_held_in_tensors_are_taken_by_value(cache, monkeypatch):
+    """A one-element tensor counts as the number it holds at the call; no size is remembered by a tensor's identity."""
+    monkeypatch.setattr(cache, "_new", lambda rows, heads: torch.zeros(rows, heads, 64, dtype=BF), raising=False)
+    sizes = []
+    real = kv4._attention_ws_bytes
+    monkeypatch.setattr(kv4, "_attention_ws_bytes", lambda *a: sizes.append(a) or real(*a) and 0)
+    calls = []
+    monkeypatch.setattr(cache, "_call", lambda fn, *a: calls.append(a), raising=False)
+    n = torch.tensor(3)
+    _call(cache, "attend", max_q=n, max_kv=torch.tensor(2000), splits=torch.tensor(2), scale=torch.tensor(0.5))
+    n += 1
+    _call(cache, "attend", max_q=n, max_kv=2000, splits=2)
+    assert [a[5:] for a in sizes] == [(3, 2000, 2), (4, 2000, 2)] and all(type(x) is int for a in sizes for x in a)
+    assert kv4._QUERY.unpack(calls[0][1])[7:] == (3, 2000, 0.5, 2)
