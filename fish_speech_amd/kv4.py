@@ -150,7 +150,8 @@ class KV4Cache:
         ``row_seq[r]``.  On the way, in this order: head RMSNorm of q and k (``q_norm`` / ``k_norm``, bf16 (head_dim,),
         llama.py:862-864), rotation of their first dims by ``rope`` (bf16 (positions, dims / 2, 2), as
         llama.py:1004-1038 builds it; pairs (2 i, 2 i + 1) or, ``rope_layout="half"``, (i, i + dims / 2)).  Returns the
-        normed and rotated q (rows, n_head, head_dim) if q was given.
+        normed and rotated q (rows, n_head, head_dim) if q was given (into ``q_out``, which may be q itself unless the
+        rotation is half-split).
 
         Rows whose sequence or position lies outside the block table (or the rotation table) are padding: nothing is
         written for them, in the cache or in ``q_out``.  A (sequence, position) pair may appear once per call."""
@@ -206,7 +207,8 @@ class KV4Cache:
         ``q_start[s] .. q_start[s + 1] - 1`` as its last positions and ``kv_len[s]`` cached keys, its own included;
         both int32 on the device, so a captured graph replays with new lengths.  ``max_q`` / ``max_kv``: upper bounds of
         one sequence's rows and keys (rows beyond ``max_q`` are not computed; ``max_kv`` only tunes the launch).  Rows
-        that see no key give 0, rows whose q holds an infinity or a NaN give NaN.  Rows behind the last sequence are left as they were in ``out`` (undefined without one).
+        that see no key give 0, rows whose q holds an infinity or a NaN give NaN.  Rows behind the last sequence are left as they were in ``out`` (undefined without one;
+        it may be q itself).
         ``splits``: key ranges per query tile, 0 = chosen from the sizes; with a fixed number (and ``max_q``) a row's bits
         do not depend on the other sequences of the call."""
         n, heads = q.shape[0], q.shape[1] if q.dim() == 3 else 0

@@ -89,8 +89,9 @@ int fmi_dualar_setup_caches(fmi_dualar* h, int max_batch, int max_seq_len);
 /* Type of the slow transformer's K/V cache: 16 = bf16 as the reference (default), 4 = the 4-bit cache described at
  * fmi_kv4_cache below: 39 168 bytes per token instead of 147 456 at 36 layers of 8 kv heads x 128 dims, for 3.76 times the
  * slots or the context in the same memory.  Keys and values then carry the rounding of that format (every query attends
- * to the stored values, also to its own token's), so logits and tokens differ from a bf16 cache's.  Call before
- * fmi_dualar_setup_caches. */
+ * to the stored values, also to its own token's), so logits and tokens differ from a bf16 cache's; prompts'
+ * softmax weights enter the product with fp16's 11 bits (fmi_op_kv4_attention below), where those of a bf16 cache have 16.
+ * Call before fmi_dualar_setup_caches. */
 int fmi_dualar_set_kv_bits(fmi_dualar* h, int bits);
 /* The stored K and V of positions [0, n) of a slot in one slow layer (4-bit cache only): bf16 [n][n_local_heads][head_dim]
  * each, after norm and rotation.  Pages of released slots may have been reused. */
@@ -294,7 +295,8 @@ int64_t fmi_kv4_page_bytes(int n_kv_head, int head_dim);
 typedef struct fmi_kv4_rows {
   const void *q_dev, *k_dev, *v_dev;   /* q_dev NULL: keys and values only */
   int64_t q_stride, k_stride, v_stride;
-  void* q_out_dev;                     /* bf16, may be q_dev itself with the same stride and no half-split rotation */
+  void* q_out_dev;                     /* bf16, may be q_dev itself with the same stride and no half-split
+                                        * rotation; overlaps none of the inputs otherwise */
   int64_t q_out_stride;
   int32_t n_head;
   const void *q_norm_dev, *k_norm_dev;
@@ -333,13 +335,15 @@ typedef struct fmi_kv4_query {
 /* Workspace fmi_op_kv4_attention needs for these sizes (0 for one key range); calls that may run at the same time need
  * workspaces of their own.  Negative for bad sizes. */
 int64_t fmi_kv4_attention_ws_bytes(const fmi_kv4_cache* cache, const fmi_kv4_query* query);
+/* out: bf16 [total_q][n_head][head_dim], rows out_stride elements apart; may be q_dev itself with the same stride. */
 int fmi_op_kv4_attention(const fmi_kv4_cache* cache, const fmi_kv4_query* query, void* out_dev, int64_t out_stride,
                          void* ws_dev, int64_t ws_bytes, void* stream);
 
 /* A generation step in one launch: fmi_op_kv4_append of `rows`, then the attention of each row's q over the keys up to its own
  * position, with the same stored bytes and the same output bits as the two calls (one query row per sequence, up to 64
  * heads per kv head) under the same `splits`.  q is required, q_out_dev is null; a sequence may have one row per call.  out: bf16
- * [rows][n_head][head_dim], rows out_stride elements apart; padding rows are left as they were.  At most 65535 rows.
+ * [rows][n_head][head_dim], rows out_stride elements apart (may be q_dev itself with the same stride); padding rows are left as they were.  At most
+ * 65535 rows.
  * Workspace: fmi_kv4_attention_ws_bytes of a query with n_seqs = total_q = rows, max_q = 1 and the same n_head, max_kv and
  * splits. */
 int fmi_op_kv4_step(const fmi_kv4_cache* cache, const fmi_kv4_rows* rows, float scale, int max_kv, int splits, void* out_dev,

@@ -173,6 +173,19 @@ def test_an_output_over_its_queries(n):
         assert torch.equal(over, want)
 
 
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_a_steps_output_over_its_queries(half, splits):
+    D, H, KVH, at = 64, 40, 1, [1300, 30]                          # 40 heads per kv head: three tiles
+    cache, t, qkv, rope, wq, wk, _, _ = setup_step(D, H, KVH, at, D, True, seed=5)
+    d, s, p, r, dq, dk = cuda(qkv, torch.arange(2, dtype=I32), torch.tensor(at, dtype=I32), rope, wq, wk)
+    q, k, v = d.split([H, KVH, KVH], dim=1)
+    kw = dict(max_kv=1301, rope=r, rope_layout="half" if half else "interleaved", q_norm=dq, k_norm=dk, splits=splits)
+    want = cache.step(q, k, v, s, p, t, **kw)
+    assert cache.step(q, k, v, s, p, t, out=q, **kw) is q
+    assert torch.equal(q, want)
+
+
 @pytest.mark.parametrize("n", [1, 40])
 def test_split_calls_on_two_streams_and_in_two_graphs(n):
     """Workspaces: two captured graphs of split calls replayed in turn and eager calls between them; two streams at once."""
