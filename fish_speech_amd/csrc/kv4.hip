@@ -466,7 +466,8 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
   constexpr int KB = 32, NT = 64 * NW, BLK = kv4_block_bytes(D), NB = D / 32;
   constexpr int KS = D / 32;                     // k-steps of a score product
   constexpr int VROW = D * 2 + 32;               // bytes of a key's row in LDS: 32 more, so that the 4 rows a 16-lane
-                                                 // group reads together lie in different banks
+                                                 // group reads together lie in different banks (the writes' conflicts:
+                                                 // 8 cycles of 18 each)
   constexpr int VL = D / 32, VP = 64 / VL;       // lanes per key and keys per pass of the V unpacking
   constexpr int VPASS = VP >= KB ? 1 : KB / VP;
   constexpr float DEFER = 8.f;
@@ -790,8 +791,9 @@ __device__ inline uint32_t kv4_pk_f16(float lo, float hi) {
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a) {
   constexpr int NT = 64 * NW, BLK = kv4_block_bytes(D), NB = D / 32, TC = 32 * NW;
-  // LDS rows: K reads take 16 keys at 16 bytes each (rows 4 banks apart), V reads 4 keys at 2 x 32 bytes (16 banks apart).
-  // V's writes then meet in a bank unless the four 16-byte words of a piece go out in an order that differs by key.
+  // LDS rows: K reads take 16 keys at 16 bytes each (rows 4 banks apart), V reads 4 keys at 2 x 32 bytes (16 banks apart), both
+  // without bank conflicts.  The writes have some: 8 cycles per 16-byte write on top of its 10, for V because the four words of
+  // a piece go out in an order that differs by key (24 in the same order).  64 of a page's 3000 cycles per wave.
   constexpr int KROW = D * 2 + 16, VROW = D * 2 + (D > 32 ? 64 : 0);
   constexpr int PIECES = 2 * KV_PAGE * NB;                  // 16-byte pieces (32 codes) of K and V of a page
   constexpr int PPT = (PIECES + NT - 1) / NT;
@@ -823,7 +825,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   // keys that all / any of the wave's columns see (a wave behind the last column sees none), and of the tile's
   int all_see = min(sp.pos0 + min(wcol, cols - 1) / G + 1, sp.cached);
   int any_see = wcol < cols ? min(sp.pos0 + min(wcol + 31, cols - 1) / G + 1, sp.cached) : 0;
-  const int tile_all = min(sp.pos0 + col0 / G + 1, sp.cached), tile_any = min(sp.pos0 + min(col0 + TC - 1, cols - 1) / G + 1, sp.cached);
+  const int tile_any = min(sp.pos0 + min(col0 + TC - 1, cols - 1) / G + 1, sp.cached);
   const int32_t* bt = a.c.block_table + (int64_t)sp.slot * a.c.max_pages;
 
   if (tid < NB) s_nan[tid] = INT32_MAX;
@@ -873,17 +875,17 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   if (pg < p_hi) fetch(page);
   __syncthreads();                                          // s_nan
   int it = 0;
-  // the pages from pg on, whose codes are in flight.  FP16: up to that of first_out; EDGE: that page alone, in fp16; BF16: the rest
-  enum { FP16, EDGE, BF16 };
-  auto pages = [&](auto phase_) {
-    constexpr int PHASE = decltype(phase_)::value;
-    constexpr bool BF = PHASE == BF16;
-    for (; pg < p_hi; ++pg, it ^= 1) {
+  // the pages from pg on, whose codes are in flight: in fp16 up to that of first_out, where the columns that see that key
+  // see nothing; in bf16
+  int p_end = p_hi;
+  auto pages = [&](auto in_bf16) {
+    constexpr bool BF = decltype(in_bf16)::value;
+    for (; pg < p_end; ++pg, it ^= 1) {
       const bool there = page >= 0 && page < a.c.n_pages;
       const int tok_end = sp.cached - pg * KV_PAGE;           // tokens of the page at or past this are not the sequence's
       uint64_t hit = 0;
       if (there) {
-        if constexpr (PHASE == FP16) {
+        if constexpr (!BF) {
           if (E < 0) {
             const int first = __builtin_amdgcn_readfirstlane((int)vtok);
             E = 0;
@@ -926,12 +928,16 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
           }
         }
       }
-      if (__builtin_expect(hit != 0, 0)) {       // (asked here, the staging does not wait for it; what is staged is staged again)
+      if (__builtin_expect(hit != 0, 0)) {       // (asked here, the staging does not wait for it)
         first_out = pg * KV_PAGE + (int)__builtin_ctzll(hit);
-        if (first_out < tile_any) return;
+        if (first_out < tile_any) {
+          p_end = pg + 1;
+          vis = seen > first_out ? 0 : seen;
+          any_see = all_see > first_out ? 0 : any_see;
+        }
       }
       __syncthreads();      // the page is staged; and every wave is done with the page before the previous one (same buffer)
-      if (PHASE != EDGE && pg + 1 < p_hi) fetch(next_page);
+      if (pg + 1 < p_end) fetch(next_page);
       if (there && pg * KV_PAGE < any_see) {
         // V^T fragments of 16 keys: lanes 4 r .. 4 r + 3 of a 16-lane group name row (key) r; lane i of the group gets dim i of
         // the 4 rows.  The first are requested before the scores, the others a product ahead.
@@ -1026,24 +1032,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
           for (int dt = 0; dt < NB; ++dt) vf[dt] = vn[dt];
         }
       }
-      if constexpr (PHASE == EDGE) {
-        it ^= 1;
-        return;
-      }
       page = next_page;
       next_page = pg + 2 < p_hi ? bt[pg + 2] : -1;
     }
   };
-  pages(std::integral_constant<int, FP16>{});
-  if (__builtin_expect(pg < p_hi && tile_all <= first_out, 0)) {
-    const int any = any_see;
-    vis = seen > first_out ? 0 : seen;
-    any_see = all_see > first_out ? 0 : any_see;
-    pages(std::integral_constant<int, EDGE>{});
-    any_see = any;
-  }
+  const int any = any_see;
+  pages(std::false_type{});
   float unit = E >= 0 ? kv4_scale((uint32_t)max(E, KV4_MIN_SCALE)) * UNLIFT : 1.f;    // of O; l's is UNLIFT
-  if (__builtin_expect(pg < p_hi, 0)) {
+  if (__builtin_expect(first_out < tile_any, 0)) {
 #pragma unroll
     for (int dt = 0; dt < NB; ++dt)
 #pragma unroll
@@ -1051,10 +1047,14 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
     l *= UNLIFT;
     unit = 1.f;
     vis = seen > first_out ? seen : 0;
+    any_see = any > first_out ? any : 0;
     all_see = all_see > first_out ? all_see : 0;
-    any_see = any_see > first_out ? any_see : 0;
+    --pg;
+    p_end = p_hi;
+    page = bt[pg];
+    next_page = pg + 1 < p_hi ? bt[pg + 1] : -1;
     fetch(page);
-    pages(std::integral_constant<int, BF16>{});
+    pages(std::true_type{});
   } else {
     l *= UNLIFT;
   }
