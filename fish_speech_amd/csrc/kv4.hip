@@ -458,8 +458,8 @@ __device__ inline float kv4_log2_scale(float scale) { return scale == 0.f ? 1.f 
 // work-group norms and rotates its own query heads (into LDS rows); the one of a kv head's last range also quantises the new
 // token's K and V, stores them, and puts them over what it fetched of that token: nothing is read back from memory, and no
 // other work-group reads that token.  The values and their bits are those of an append followed by an attention.  In a
-// captured graph 8 x 300 keys take 8.4 us where the two launches take 9.5, 16 x 1k 12.7 and 14.3, 32 x 6k 49 and 53; a
-// model's frame of 36 layers went from 4.15 to 4.10 ms at 200 tokens, the host's part of a call pair from 17.6 to 10.2 us.
+// captured graph 8 x 300 keys take 8.5 us where the two launches take 9.7, 16 x 1k 13.0 and 14.3, 32 x 6k 50 and 51; a
+// model's frame of 36 layers went from 4.15 to 4.09 ms at 200 tokens, the host's part of a call pair from 18.4 to 10.6 us.
 struct Kv4None {};
 template <int D, int NW, int STEP>
 __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::conditional_t<STEP != 0, Kv4AppendArgs, Kv4None> p) {
@@ -765,11 +765,12 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
 // From the first key on that has another power (`first_out`; an all-zero block has the smallest there is), the rows that see
 // it go on in bf16, whose powers are fp32's: V exact, the weights as high and low part (16 bits), a second product.  The page
 // of that key is taken twice, for the rows before it in fp16 and for those from it on in bf16; what a row gives depends on no
-// key behind it, on no other row and not on the tile that it is in.  All in bf16 from the start: 18 to 22 % more time on
-// prompts of 2k tokens (8 over 4k keys 1.42 -> 1.73 ms), 7 % on 200.
-// Bound by issue: per page and wave 32 matrix instructions (34 % of the time) and 260 others (43 %), two waves per SIMD to
-// overlap them.  8 prompts of 2k tokens over 4k keys run at 960 TFLOP/s, two ragged ones at 850 (222 us; the last
-// work-groups run alone), 8 ragged prompts of up to 200 tokens in 14.5 us, mostly the latency of their 1 to 4 pages.
+// key behind it, on no other row and not on the tile that it is in.  fp16 / bf16 from the first page on: 8 prompts of 2k tokens
+// over 4k keys 1382 / 1760 us, two ragged ones 246 / 281, 8 ragged prompts of up to 200 tokens 15.9 / 19.0.
+// Bound by issue: per page and wave 32 matrix instructions (34 % of the time) and 245 others (42 %), two waves per SIMD to
+// overlap them.  8 prompts of 2k tokens over 4k keys run at 990 TFLOP/s, two ragged ones at 860 (220 us where calls come one by
+// one, 246 without a pause between them; the last work-groups run alone), 8 ragged prompts of up to 200 tokens in 14.7 us,
+// mostly the latency of their 1 to 4 pages.
 // The native product of 4-bit K with Q in two 8-bit parts needs no unpacking and the same matrix time, but its sums came out
 // 9e-5 of the absolute sum away from the exact ones (bf16 products: 1e-7), too coarse for scores.
 typedef __attribute__((ext_vector_type(8))) _Float16 f16x8_t;
