@@ -440,6 +440,11 @@ __device__ inline void kv4_prepare_q(u32x4& t, float scale) {
 // scores in units of log2
 __device__ inline float kv4_log2_scale(float scale) { return scale == 0.f ? 1.f : fabsf(scale) * 1.4426950408889634f; }
 
+// A running reference r of a softmax whose weights are 2^(s sl - r), set when its largest score reaches mx: `above` it, and by two
+// steps of mx more, so that no weight exceeds 2^-above whatever the rounding of large scores.  r itself goes into every weight and
+// into every change of reference: both round alike.
+__device__ inline float kv4_reference(float mx, float above) { return fmaf(fabsf(mx), 0x1p-22f, mx + above); }
+
 // ---- few query columns: tiles of 16, the kernel of single tokens.  NW waves; wave w takes the 32-key blocks w, w + NW, ...
 // of the range.  Per block:
 //   scores   S^T = K Q^T, v_mfma_f32_16x16x32_bf16: lane (c, g) holds the D / 4 dims from g D / 4 of key c, which is one
@@ -470,7 +475,6 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
                                                  // 8 cycles of 18 each)
   constexpr int VL = D / 32, VP = 64 / VL;       // lanes per key and keys per pass of the V unpacking
   constexpr int VPASS = VP >= KB ? 1 : KB / VP;
-  constexpr float DEFER = 8.f;
   __shared__ __attribute__((aligned(16))) unsigned char s_v[NW][KB * VROW];
   __shared__ float s_m[NW][16], s_l[NW][16];
   __shared__ int s_nan[NW][NB];
@@ -662,12 +666,12 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) mx = fmaxf(mx, t[i]);
-      mx = max_swap32(max_swap16(mx)) * sl;
-      // the reference m moves only when a score exceeds it by 2^8: O is seldom rescaled.  Weights are relative to the most it
-      // can be exceeded by, so none is above 1 and O no larger than with the true maximum (V may be as large as 2^127).
-      const float mn = mx > m + DEFER ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn), top = mn + DEFER;
+      mx = max_swap32(max_swap16(mx));
+      // the reference m lies 2^8 above the largest score when it moves, and moves when a score exceeds it: O is seldom rescaled, no
+      // weight is above 1 and O no larger than with the true maximum (V may be as large as 2^127)
+      const float mn = fmaf(mx, sl, -m) > 0.f ? kv4_reference(mx * sl, 8.f) : m, corr = __builtin_amdgcn_exp2f(m - mn);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f(fmaf(t[i], sl, -top));
+      for (int i = 0; i < 8; ++i) t[i] = __builtin_amdgcn_exp2f(fmaf(t[i], sl, -mn));
       l = l * corr + (((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7])));
       m = mn;
       u32x4 ph, pl;
@@ -754,10 +758,10 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
 //   scores   S^T = K Q^T, v_mfma_f32_32x32x16_bf16, Q in registers for the whole kernel;
 //   softmax  as above; the probabilities are rounded to fp16 (11 bits: with bf16's 8 a second product with the remainder
 //            would be needed, half as much matrix work again) and stay in registers.  fp16 has few powers of two, so all of
-//            them are used: probabilities are formed times 2^10, the reference m moves at 2^5, the largest is 2^15.  11 bits
-//            then hold down to 2^-24 of the reference's weight, and only what is under 2^-35 of it rounds to 0 (unlifted: 2^-14
-//            and 2^-25, which is where the keys beside an attention sink lie).  Moving m at 2^3 costs 2 % more (rescales),
-//            at 2^8 nothing less;
+//            them are used: the largest probability is 2^10 when the reference m is set and m moves when one would pass 2^15.
+//            11 bits then hold down to 2^-24 of the largest, and only what is under 2^-35 of it rounds to 0 (around 1: 2^-14
+//            and 2^-25, which is where the keys beside an attention sink lie).  2^3 between the two instead of 2^5 costs 2 %
+//            more (rescales), 2^8 nothing less;
 //   output   O^T += V^T P, v_mfma_f32_32x32x16_f16, V^T by ds_read_b64_tr_b16.
 // V is held in fp16 relative to 2^E, E = the largest block power of the range's first key, which every row sees that sees
 // any key of it.  fp16 is sound only while powers are alike: while every block's is within 2^-4 .. 2^5 of 2^E, V is exact and
@@ -798,7 +802,7 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   constexpr int KROW = D * 2 + 16, VROW = D * 2 + (D > 32 ? 64 : 0);
   constexpr int PIECES = 2 * KV_PAGE * NB;                  // 16-byte pieces (32 codes) of K and V of a page
   constexpr int PPT = (PIECES + NT - 1) / NT;
-  constexpr float DEFER = 5.f, LIFT = 10.f, UNLIFT = 0x1p-15f;   // powers of two: see "softmax" above
+  constexpr float DEFER = 5.f, TOP = 15.f;                  // powers of two: see "softmax" above
   constexpr uint32_t BELOW = 4, ABOVE = 5;                  // V's powers around E
   __shared__ __attribute__((aligned(16))) unsigned char s_k[2][KV_PAGE * KROW];
   __shared__ __attribute__((aligned(16))) unsigned char s_v[2][KV_PAGE * VROW];
@@ -983,14 +987,15 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
           for (int i = 0; i < 16; ++i) mx = fmaxf(mx, sacc[kt][i]);
-        mx = max_swap32(mx) * sl;
-        // the reference m moves only when a score exceeds it by 2^5: O is seldom rescaled
-        const float mn = mx > m + DEFER ? mx : m, corr = __builtin_amdgcn_exp2f(m - mn), lift = (BF ? -DEFER : LIFT) - mn;
+        mx = max_swap32(mx);
+        // weights are at most 2^TOP; the reference m moves when one would exceed that, DEFER beyond: O is seldom rescaled
+        constexpr float MOST = BF ? 0.f : TOP;
+        const float mn = fmaf(mx, sl, -m) > MOST ? kv4_reference(mx * sl, DEFER - MOST) : m, corr = __builtin_amdgcn_exp2f(m - mn);
         float ps = 0.f;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) sacc[kt][i] = __builtin_amdgcn_exp2f(fmaf(sacc[kt][i], sl, lift));
+          for (int i = 0; i < 16; ++i) sacc[kt][i] = __builtin_amdgcn_exp2f(fmaf(sacc[kt][i], sl, -mn));
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll
@@ -1039,13 +1044,16 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
   };
   const int any = any_see;
   pages(std::false_type{});
-  float unit = E >= 0 ? kv4_scale((uint32_t)max(E, KV4_MIN_SCALE)) * UNLIFT : 1.f;    // of O; l's is UNLIFT
+  // from here on weights of at most 1, and O in units of 1
+  const float top = m + TOP, down = __builtin_amdgcn_exp2f(m - top);
+  float unit = E >= 0 ? kv4_scale((uint32_t)max(E, KV4_MIN_SCALE)) * down : 1.f;
+  m = top;
+  l *= down;
   if (__builtin_expect(first_out < tile_any, 0)) {
 #pragma unroll
     for (int dt = 0; dt < NB; ++dt)
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[dt][i] *= unit;
-    l *= UNLIFT;
     unit = 1.f;
     vis = seen > first_out ? seen : 0;
     any_see = any > first_out ? any : 0;
@@ -1056,8 +1064,6 @@ __global__ __launch_bounds__(64 * NW, 2) void kv4_attn_wide_kernel(Kv4AttnArgs a
     next_page = pg + 1 < p_hi ? bt[pg + 1] : -1;
     fetch(page);
     pages(std::true_type{});
-  } else {
-    l *= UNLIFT;
   }
 
   l = sum_swap32(l);

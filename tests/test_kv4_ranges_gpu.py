@@ -215,3 +215,28 @@ def test_sums_of_large_and_small_values_stay_in_range(D, H, KVH, rows, power):
     ref, tol = reference(q, ks, vs, scale, weight_bits(rows, H // KVH))
     for splits in (1, 3):
         assert worst(attend(cache, t, q, keys, splits, scale=scale), ref, tol) <= 1, splits
+
+
+@pytest.mark.parametrize("base, step", [(0.0, 2), (2.0 ** 20, 2), (2.0 ** 24, 2), (2.0 ** 25, 4), (2.0 ** 26, 8), (2.0 ** 27, 16), (-2.0 ** 25, 4), (-2.0 ** 27, 16)])
+@pytest.mark.parametrize("rows", [1, 16, 70])
+@pytest.mark.parametrize("splits", [1, 3])
+def test_scores_so_large_that_fp32_rounds_their_exponents(base, step, rows, splits):
+    """Scores base + a few steps, exact in fp32, that grow along the keys: the weights depend on the differences alone."""
+    D, H, KVH, keys = 64, 4, 2, 1500
+    scale = math.log(2)
+    q, k = torch.zeros(rows, H, D), torch.zeros(keys, KVH, D)
+    q[..., 0], q[..., 32] = base, 1.0
+    k[..., 0] = 1.0
+    g = torch.Generator().manual_seed(2)
+    grid = torch.tensor([0.0, 2, 4, 6, 8, 12, 16, 24])              # (one power for the block: its largest value is in every row)
+    grid = grid[(grid % step) == 0]
+    pick = (torch.rand(keys, KVH, generator=g) * (1 + torch.arange(keys)[:, None] / keys * (len(grid) - 1))).long()
+    k[..., 32], k[..., 33] = grid[pick], 24.0
+    v = 1 + randn(keys, KVH, D, seed=3).float() * 0.3
+    cache, t, ks, vs = stored_cache(k.to(BF), v.to(BF))
+    assert torch.equal(ks, k.double())
+    ref, _ = reference(q.to(BF), ks, vs, scale, 0.0)
+    bits = weight_bits(rows, H // KVH)
+    # the scores are exact, their product with the scale in units of log2 is off by a common factor: half a step of 24 at most
+    tol = 2.0 ** -8 * ref.abs() + (bits + 2.0 ** -16 + keys * 2.0 ** -24) * vs.abs().max()
+    assert worst(attend(cache, t, q.to(BF), keys, splits, scale=scale), ref, tol) <= 1
