@@ -463,8 +463,8 @@ __device__ inline float kv4_reference(float mx, float above) { return fmaf(fabsf
 // work-group norms and rotates its own query heads (into LDS rows); the one of a kv head's last range also quantises the new
 // token's K and V, stores them, and puts them over what it fetched of that token: nothing is read back from memory, and no
 // other work-group reads that token.  The values and their bits are those of an append followed by an attention.  In a
-// captured graph 8 x 300 keys take 8.5 us where the two launches take 9.7, 16 x 1k 13.0 and 14.3, 32 x 6k 50 and 51; a
-// model's frame of 36 layers went from 4.15 to 4.09 ms at 200 tokens, the host's part of a call pair from 18.4 to 10.6 us.
+// captured graph 8 x 300 keys take 8.5 us where the two launches take 9.7, 16 x 1k 13.1 and 14.3, 32 x 6k 50 and 52; a
+// model's frame of 36 layers went from 4.15 to 4.09 ms at 200 tokens, the host's part of a call pair from 18.8 to 10.8 us.
 struct Kv4None {};
 template <int D, int NW, int STEP>
 __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::conditional_t<STEP != 0, Kv4AppendArgs, Kv4None> p) {
@@ -770,9 +770,9 @@ __global__ __launch_bounds__(64 * NW) void kv4_attn_kernel(Kv4AttnArgs a, std::c
 // it go on in bf16, whose powers are fp32's: V exact, the weights as high and low part (16 bits), a second product.  The page
 // of that key is taken twice, for the rows before it in fp16 and for those from it on in bf16; what a row gives depends on no
 // key behind it, on no other row and not on the tile that it is in.  fp16 / bf16 from the first page on: 8 prompts of 2k tokens
-// over 4k keys 1382 / 1760 us, two ragged ones 246 / 281, 8 ragged prompts of up to 200 tokens 15.9 / 19.0.
+// over 4k keys 1431 / 1805 us, two ragged ones 246 / 284, 8 ragged prompts of up to 200 tokens 15.6 / 18.6.
 // Bound by issue: per page and wave 32 matrix instructions (34 % of the time) and 245 others (42 %), two waves per SIMD to
-// overlap them.  8 prompts of 2k tokens over 4k keys run at 990 TFLOP/s, two ragged ones at 860 (220 us where calls come one by
+// overlap them.  8 prompts of 2k tokens over 4k keys run at 960 TFLOP/s, two ragged ones at 850 (224 us where calls come one by
 // one, 246 without a pause between them; the last work-groups run alone), 8 ragged prompts of up to 200 tokens in 14.7 us,
 // mostly the latency of their 1 to 4 pages.
 // The native product of 4-bit K with Q in two 8-bit parts needs no unpacking and the same matrix time, but its sums came out
